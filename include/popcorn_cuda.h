@@ -105,7 +105,8 @@ PC_API int pc_memcpy_dtoh_async(void* dst, const void* src, size_t bytes, void* 
 PC_API int pc_stream_synchronize(void* stream);
 /* Reads and clears the device-side error word of `device` (bit 0: a bounded
  * wait inside a kernel gave up; bit 1: a decode position outside the cache;
- * bit 4: an embedding id outside the table). 0 when clean. Synchronises the
+ * bit 4: an embedding id outside the table; bit 5: a page id outside the
+ * pages). 0 when clean. Synchronises the
  * device. */
 PC_API int pc_device_error_check(int device, uint32_t* flags);
 
@@ -429,6 +430,85 @@ PC_API int pc_kernel_embedding_gather_affine_quantized(const pc_tensor* ids, con
                                                        int64_t vocab, int64_t hidden, int32_t bits,
                                                        int32_t group_size, const pc_tensor* out,
                                                        pc_kernel** kernel);
+
+/* ---- a paged serving step (extensions) ------------------------------------ */
+
+/* One step of a server with many requests: R requests (at most 16384), each
+ * with keys in a cache of pages and new tokens of this step, packed one
+ * request after the other into T token rows. The four kernels below read
+ * every length from device memory, so one captured CUDA graph serves steps
+ * of any lengths that fit its tensors. Pages are [P, Nkv, ps, Hd]; row j of
+ * request r is row j % ps of page block_table[r, j / ps]. All index tensors
+ * are int32. No output may overlap another tensor of its call, but where it
+ * is said. */
+
+/* Block table, slot map and token positions of a step, from the requests'
+ * lengths: request r has cached[r] keys and adds added[r] tokens (negative
+ * lengths count as 0). The pages that it needs beyond those it has,
+ * ceil((cached + added) / ps) - ceil(cached / ps), are taken from free_pages
+ * [F] at *free_head (clamped to [0, F]) on, in request order, and entered
+ * into block_table [R, W] behind those of its cached keys; other entries
+ * stay. The first request that does not fit (free pages, W, the T token
+ * rows, 2^31 - 1 keys), and all after it, wait: they add no token in this
+ * step. Written: seq_lens [R] = keys after the step; query_start [R + 1] =
+ * first token row of each request, the last one the total; positions and
+ * slots [T] = each token's position and page * ps + row (-1 where a page id
+ * is negative), 0 and -1 in the rows after the last token; last_rows [R] =
+ * the row before query_start[r + 1] (0 when there is none); free_head_out
+ * [1]; admitted [1] = the number of requests that did not have to wait.
+ * seq_lens may be cached and free_head_out may be free_head: a loop of steps
+ * then keeps its state on the device. */
+PC_API int pc_kernel_paged_batch_build(const pc_tensor* cached, const pc_tensor* added, const pc_tensor* free_pages,
+                                       const pc_tensor* free_head, const pc_tensor* block_table, int64_t page_size,
+                                       const pc_tensor* seq_lens, const pc_tensor* query_start,
+                                       const pc_tensor* positions, const pc_tensor* slots, const pc_tensor* last_rows,
+                                       const pc_tensor* free_head_out, const pc_tensor* admitted, pc_kernel** kernel);
+/* Splits qkv [T, (Nq+2*Nkv)*Hd] (ONE Matmul against the concatenated [W_q;
+ * W_k; W_v]) into q_out [T,Nq,Hd] and the key / value rows of the pages at
+ * slots [T] (page * ps + row; distinct; a slot outside the pages writes no
+ * key / value row). On the way, optionally: RMSNorm of each q and k head
+ * (qk_norm; weights q_norm / k_norm f32 [Hd] or NULL, as (1 + w) with
+ * add_one_to_weight) and of each v head without weight (norm_v), then
+ * rotate-half RoPE of q and k with f32 tables cos / sin [T, Hd/2], one row a
+ * token (both or none). fp32 arithmetic, one rounding at the store; heads
+ * with neither are copied bit for bit. One float dtype. */
+PC_API int pc_kernel_paged_qkv_scatter(const pc_tensor* qkv, const pc_tensor* slots, const pc_tensor* q_out,
+                                       const pc_tensor* k_pages, const pc_tensor* v_pages, const pc_tensor* cos_t,
+                                       const pc_tensor* sin_t, int32_t qk_norm, const pc_tensor* q_norm,
+                                       const pc_tensor* k_norm, int32_t norm_v, float eps, int32_t add_one_to_weight,
+                                       pc_kernel** kernel);
+/* Attention of the step's new tokens over the pages: q, out [T,Nq,Hd]; token
+ * i of request r (rows query_start[r].. of q) sits at position seq_lens[r] -
+ * n + i, n = query_start[r+1] - query_start[r], and attends to its request's
+ * keys: causal j <= position; sliding window also position - j < window, or
+ * j < sinks (the first `sinks` tokens stay visible; sinks > 0 only with that
+ * mask); bidirectional all. KV head hq * Nkv / Nq, Hd <= 512, one float
+ * dtype. fp32 softmax and accumulation; a row without a visible key is zero;
+ * rows of no request are left as they are. Values in keys that a row does
+ * not see never reach it, whatever they are. Lengths are clamped to the
+ * tensors on the device; a page id outside the pages is never read: it sets
+ * bit 5 of the device error word and its request's rows hold no meaningful
+ * result. */
+PC_API int pc_kernel_paged_attention(const pc_tensor* q, const pc_tensor* k_pages, const pc_tensor* v_pages,
+                                     const pc_tensor* block_table, const pc_tensor* seq_lens,
+                                     const pc_tensor* query_start, const pc_tensor* out, float scale,
+                                     pc_attention_mask mask, int32_t sinks, pc_kernel** kernel);
+/* The next token of each row of logits [.., V] (f32, f16, bf16) from one
+ * given random number uniform [rows] in [0, 1), f32. With w_i = exp((l_i -
+ * l_max) / temperature) and tokens ordered by (logit descending, index
+ * ascending): top_k (i32; <= 0 or >= V: off) keeps the first k; top_p (f32;
+ * >= 1 or NaN: off) the shortest prefix of those whose weight reaches top_p
+ * times theirs, one at least; min_p (f32; <= 0 or NaN: off) those with w_i
+ * >= min(min_p, 1). The token is the first index, in index order, at which
+ * the running weight of the kept tokens exceeds uniform times their whole
+ * weight. temperature (f32) <= 0 or NaN: the largest logit, lowest index.
+ * Each of the four is [rows] or NULL (temperature 1, off). NaN logits count
+ * as -inf; -inf is never drawn; a row of nothing else gives -1. Weights and
+ * their sums are 42-bit fixed point, so the result does not depend on the
+ * order of additions; tokens below 2^-43 of the largest are never drawn. */
+PC_API int pc_kernel_sample(const pc_tensor* logits, const pc_tensor* uniform, const pc_tensor* tokens,
+                            const pc_tensor* temperature, const pc_tensor* top_k, const pc_tensor* top_p,
+                            const pc_tensor* min_p, pc_kernel** kernel);
 
 /* ---- tensor parallelism over peer memory (extension) ---------------------- */
 

@@ -153,6 +153,10 @@ def _declare(L):
                                                    I),
         "pc_kernel_gated_activation": ([T, I32, T, PP], I),
         "pc_kernel_add_rmsnorm": ([T, T, T, F, I32, T, T, PP], I),
+        "pc_kernel_paged_batch_build": ([T, T, T, T, T, I64, T, T, T, T, T, T, T, PP], I),
+        "pc_kernel_paged_qkv_scatter": ([T, T, T, T, T, T, T, I32, T, T, I32, F, I32, PP], I),
+        "pc_kernel_paged_attention": ([T, T, T, T, T, T, T, F, M, I32, PP], I),
+        "pc_kernel_sample": ([T, T, T, T, T, T, T, PP], I),
         "pc_flash_decoding_noalloc": ([T, T, T, T, T, F, M, P], I),
         "pc_flash_decoding_noalloc_capacity": ([], ctypes.c_size_t),
         "pc_decode_stack_workspace_bytes": ([ctypes.POINTER(pc_decode_stack_desc), ctypes.POINTER(ctypes.c_uint64)], I),

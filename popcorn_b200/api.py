@@ -720,6 +720,59 @@ class Kernels:
                              _tc(sum_out), _tc(norm_out), keep=_keep(group, residual, norm_weight, sum_out, norm_out))
 
 
+class _PagedBatchBuild(Kernel):
+    """Extension: block table, slot map and token positions of a paged step
+    from the requests' lengths (pc_kernel_paged_batch_build). seq_lens may be
+    `cached` and free_head_out may be `free_head` (state kept in place)."""
+
+    def __init__(self, cached, added, free_pages, free_head, block_table, page_size, seq_lens, query_start, positions,
+                 slots, last_rows, free_head_out, admitted):
+        ts = (cached, added, free_pages, free_head, block_table, seq_lens, query_start, positions, slots, last_rows,
+              free_head_out, admitted)
+        super().__init__(N.lib().pc_kernel_paged_batch_build, *[_tc(t) for t in ts[:5]], int(page_size),
+                         *[_tc(t) for t in ts[5:]], keep=_keep(*ts))
+
+
+class _PagedQKVScatter(Kernel):
+    """Extension: q rows and K/V page rows out of one fused QKV Matmul, with
+    the optional per-head norms and RoPE (pc_kernel_paged_qkv_scatter)."""
+
+    def __init__(self, qkv, slots, q_out, k_pages, v_pages, cos=None, sin=None, qk_norm=False, q_norm=None,
+                 k_norm=None, norm_v=False, eps=1e-6, add_one_to_weight=False):
+        super().__init__(N.lib().pc_kernel_paged_qkv_scatter, _tc(qkv), _tc(slots), _tc(q_out), _tc(k_pages),
+                         _tc(v_pages), _tc(cos), _tc(sin), int(qk_norm), _tc(q_norm), _tc(k_norm), int(norm_v),
+                         ctypes.c_float(eps), int(add_one_to_weight),
+                         keep=_keep(qkv, slots, q_out, k_pages, v_pages, cos, sin, q_norm, k_norm))
+
+
+class _PagedAttention(Kernel):
+    """Extension: attention of a step's new tokens (one or a chunk per
+    request) over a paged cache; `sinks` first tokens stay visible under a
+    sliding-window mask (pc_kernel_paged_attention)."""
+
+    def __init__(self, q, k_pages, v_pages, block_table, seq_lens, query_start, into, scale,
+                 mask=AttentionMask.causal, sinks=0):
+        super().__init__(N.lib().pc_kernel_paged_attention, _tc(q), _tc(k_pages), _tc(v_pages), _tc(block_table),
+                         _tc(seq_lens), _tc(query_start), _tc(into), ctypes.c_float(scale), mask.c(), int(sinks),
+                         keep=_keep(q, k_pages, v_pages, block_table, seq_lens, query_start, into))
+
+
+class _Sample(Kernel):
+    """Extension: the next token of each row of logits by temperature, top-k,
+    top-p, min-p and a given random number (pc_kernel_sample)."""
+
+    def __init__(self, logits, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None):
+        super().__init__(N.lib().pc_kernel_sample, _tc(logits), _tc(uniform), _tc(tokens), _tc(temperature),
+                         _tc(top_k), _tc(top_p), _tc(min_p),
+                         keep=_keep(logits, uniform, tokens, temperature, top_k, top_p, min_p))
+
+
+Kernels.PagedBatchBuild = _PagedBatchBuild
+Kernels.PagedQKVScatter = _PagedQKVScatter
+Kernels.PagedAttention = _PagedAttention
+Kernels.Sample = _Sample
+
+
 class _MatmulAllReduceAddRMSNorm(Kernel):
     """Extension: Matmul (a . w^T, M <= 64, tensor cores) into this rank's
     PeerGroup partial buffer, then the all-reduce + Add + RMSNorm, in ONE

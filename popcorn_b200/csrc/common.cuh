@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace popcorn {
 namespace launch {
 
@@ -35,6 +37,46 @@ cudaError_t launch_k(F kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t 
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+
+// As launch_k, with the grid in clusters of `cluster` CTAs along x.
+template <class F, class... Args>
+cudaError_t launch_cluster(F kernel, dim3 grid, dim3 block, unsigned cluster, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Runs a kernel's set-up once per device (function attributes belong to the
+// device that is current when they are set).
+class DeviceOnce {
+public:
+    template <class F>
+    cudaError_t run(F setup) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = uint64_t(1) << (dev & 63);
+        if (done_.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = setup();
+        if (e == cudaSuccess) done_.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+
+private:
+    std::atomic<uint64_t> done_{0};
+};
 
 // Raises a kernel's dynamic shared memory limit once per process.
 template <class F>

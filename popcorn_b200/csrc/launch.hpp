@@ -288,6 +288,73 @@ struct Argmax {
 void argmax_plan(Argmax& p, int sm_count);
 cudaError_t argmax(const Argmax& p, cudaStream_t stream);
 
+// The paged serving step (paged.cu, paged_attention.cu, sample.cu).
+constexpr int kMaxRequests = 16384;  // of one step: their lengths' prefix sums stay in shared memory
+struct PagedBatch {
+    const int32_t* cached;      // [R] tokens in the cache before the step
+    const int32_t* added;       // [R] tokens that the step adds
+    const int32_t* free_pages;  // [F] free page ids, taken from *free_head on
+    const int32_t* free_head;   // [1]
+    int32_t* table;             // [R, W]
+    int32_t* seq_lens;          // [R]
+    int32_t* query_start;       // [R + 1]
+    int32_t* positions;         // [T]
+    int32_t* slots;             // [T]
+    int32_t* last_rows;         // [R]
+    int32_t* free_head_out;     // [1]
+    int32_t* admitted;          // [1]
+    int R;
+    int64_t W, F, T, ps;
+    int ctas;  // set at launch
+};
+cudaError_t paged_batch_build(const PagedBatch& p, cudaStream_t stream);
+struct PagedScatter {
+    const void* qkv;       // [T, (Nq + 2 Nkv) * Hd]
+    const int32_t* slots;  // [T]; outside [0, P * ps): no K/V row is written
+    void* q_out;           // [T, Nq, Hd]
+    void* k_pages;         // [P, Nkv, ps, Hd]
+    void* v_pages;
+    const float* cos_t;  // [T, Hd / 2] or null
+    const float* sin_t;
+    const float* q_norm;  // [Hd] or null
+    const float* k_norm;
+    int dtype;
+    int64_t T, P, ps, Hd;
+    int Nq, Nkv;
+    int qk_norm, norm_v, add_one;
+    float eps;
+};
+cudaError_t paged_qkv_scatter(const PagedScatter& p, cudaStream_t stream);
+struct PagedAttention {
+    const void* q;  // [T, Nq, Hd]
+    const void* k_pages;  // [P, Nkv, ps, Hd]
+    const void* v_pages;
+    const int32_t* table;        // [R, W]
+    const int32_t* seq_lens;     // [R] keys of each request, the new ones included
+    const int32_t* query_start;  // [R + 1]
+    void* out;  // [T, Nq, Hd]
+    int dtype;
+    int64_t T, P, ps, Hd, W;
+    int R, Nq, Nkv;
+    float scale;
+    int mask_kind;
+    int32_t window, sinks;
+};
+// The form for every type, head dim, page size and alignment.
+cudaError_t paged_attention_any(const PagedAttention& p, cudaStream_t stream);
+struct Sample {
+    const void* logits;  // [rows, V]
+    int dtype;
+    const float* uniform;      // [rows]
+    const float* temperature;  // [rows] or null (1)
+    const int32_t* top_k;      // [rows] or null (off)
+    const float* top_p;        // [rows] or null (off)
+    const float* min_p;        // [rows] or null (off)
+    int32_t* tokens;           // [rows]
+    int64_t rows, V;
+};
+cudaError_t sample(const Sample& p, cudaStream_t stream);
+
 // One-shot all-reduce of tensor-parallel partial sums over peer memory,
 // fused with the residual add and RMSNorm (allreduce.cu).
 constexpr int kMaxPeers = 8;

@@ -1501,6 +1501,11 @@ int wrap(std::unique_ptr<Kernel> k, pc_kernel** out) {
 }
 }  // namespace
 
+// Used by paged_ops.cu for its half of the ABI.
+namespace popcorn {
+int make_kernel(std::unique_ptr<Kernel> k, pc_kernel** out) { return wrap(std::move(k), out); }
+}  // namespace popcorn
+
 #define PC_GUARD_BEGIN                       \
     try {                                    \
         if (kernel) *kernel = nullptr;
