@@ -212,6 +212,12 @@ class KernelScratchAllocator:
         pass
 
     def _c(self):
+        # one pair of callbacks for every encoder over this allocator: an
+        # encoder holds their addresses as long as it lives
+        cb = getattr(self, "_cb", None)
+        if cb is not None:
+            return N.pc_scratch_allocator(None, cb[0], cb[1])
+
         def _borrow(ctx, length, out_ptr, out_reused):
             try:
                 ptr, reused = self.borrow(int(length))

@@ -196,3 +196,23 @@ def test_sample_refusals(change, code):
 def test_sample_refuses_overlap():
     a = sample_args()
     refused(E.tensorShapeMismatch, pc.Kernels.Sample, **dict(a, tokens=a["top_k"]))
+
+
+def test_encoders_share_an_allocator():
+    """An allocator's callbacks live as long as it does: a second encoder over it leaves the first's in place."""
+    import ctypes
+    import gc
+
+    class Fixed(pc.KernelScratchAllocator):
+        def borrow(self, length):
+            return 4096 + length, False
+
+    pool = Fixed()
+    first = pool._c()
+    addresses = [ctypes.cast(getattr(first, n), ctypes.c_void_p).value for n in ("borrow", "release")]
+    second = pool._c()
+    gc.collect()
+    assert [ctypes.cast(getattr(second, n), ctypes.c_void_p).value for n in ("borrow", "release")] == addresses
+    out, reused = ctypes.c_void_p(), ctypes.c_int()
+    for st in (first, second):
+        assert st.borrow(None, 64, ctypes.byref(out), ctypes.byref(reused)) == 0 and out.value == 4160
