@@ -342,6 +342,17 @@ struct PagedAttention {
 };
 // The form for every type, head dim, page size and alignment.
 cudaError_t paged_attention_any(const PagedAttention& p, cudaStream_t stream);
+// The tensor-core form: `ctas` CTAs share the step's work; the pieces of what
+// they cut are joined by a second launch.
+struct PagedScratch {
+    void* base;  // paged_attention_scratch_bytes
+    int ctas;
+};
+bool paged_attention_tc_supports(const PagedAttention& p);
+int64_t paged_attention_scratch_rows(const PagedAttention& p);
+size_t paged_attention_scratch_bytes(const PagedAttention& p, int ctas);
+cudaError_t paged_attention_tc(const PagedAttention& p, const PagedScratch& scratch, cudaStream_t stream);
+cudaError_t paged_attention_join(const PagedAttention& p, const PagedScratch& scratch, cudaStream_t stream);
 struct Sample {
     const void* logits;  // [rows, V]
     int dtype;

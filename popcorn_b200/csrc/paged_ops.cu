@@ -211,19 +211,36 @@ public:
         p_ = launch::PagedAttention{q.data(), k.data(), v.data(), ptr<int32_t>(table), ptr<int32_t>(seq_lens),
                                     ptr<int32_t>(query_start), out.data(), dt, T, P, ps, Hd, W, int(R), int(Nq), int(Nkv),
                                     scale, mask.kind, mask.window, sinks};
-        function_names_ = std::string("paged_attention") + tag(dt);
+        tc_ = launch::paged_attention_tc_supports(p_);
+        function_names_ = std::string("paged_attention") + (tc_ ? "_tc" : "") + tag(dt);
+        if (tc_) function_names_ += std::string(";paged_attention_join") + tag(dt);
     }
     const char* name() const override { return "PagedAttention"; }
     std::vector<Binding> tensors() const override { return b_; }
     void encode(KernelCommandEncoder& enc) const override {
         launch::PagedAttention p = p_;
         if (p.T == 0 || p.R == 0) return;
-        enc.dispatch(function_names_, b_, [p](cudaStream_t s) { return launch::paged_attention_any(p, s); });
+        if (!tc_) {
+            enc.dispatch(function_names_, b_, [p](cudaStream_t s) { return launch::paged_attention_any(p, s); });
+            return;
+        }
+        const int ctas = enc.sm_count();
+        const int64_t words = int64_t((launch::paged_attention_scratch_bytes(p, ctas) + 3) / 4);
+        enc.with_temporaries({{{words}, PC_F32}}, [&](const std::vector<Tensor>& t) {
+            const launch::PagedScratch sc{t[0].data(), ctas};
+            std::vector<Binding> first = b_;
+            first.push_back({t[0], PC_ACCESS_WRITE});
+            enc.dispatch(std::string("paged_attention_tc") + tag(p.dtype), first,
+                         [p, sc](cudaStream_t s) { return launch::paged_attention_tc(p, sc, s); });
+            enc.dispatch(std::string("paged_attention_join") + tag(p.dtype), {{t[0], PC_ACCESS_READ}, {b_.back().tensor, PC_ACCESS_WRITE}},
+                         [p, sc](cudaStream_t s) { return launch::paged_attention_join(p, sc, s); });
+        });
     }
 
 private:
     std::vector<Binding> b_;
     launch::PagedAttention p_{};
+    bool tc_ = false;
 };
 
 // ---------------------------------------------------------------------------
