@@ -13,16 +13,16 @@
 // alone, so results repeat bit for bit). The plan is computed by every CTA
 // from the lengths on the device.
 //
-// In a CTA: warp 0 loads Q and the 64-key halves of K and V tiles by TMA
-// (128-byte swizzle, one box per page run) into one ring in the order K(0),
-// K(1) V(0), K(2) V(1), ...; warp 1 issues S = Q.K^T into the next of NS
-// accumulators in tensor memory and O += P.V, whichever is ready; warps 4-11
-// (two threads a row, 64 keys each) turn S into P = 2^(c S - m): P is packed
-// into the type and written back over S, from where the second product reads
-// it as its A operand, so it never passes through shared memory. A ring slot
-// holds 8-key groups of [Hd/64][8 keys][128 B], so any page size that is a
-// multiple of 8 gives one layout (group stride Hd/64 KB) and 128 keys in
-// neighbouring slots are one operand.
+// In a CTA: warp 0 walks the items, looks pages up and loads Q and K by TMA
+// (128-byte swizzle, a box per run of page rows); warp 2 loads V; both fill
+// one ring in the order K(0), K(1), V(0), K(2), V(1), ...; warp 1 issues S = Q.K^T
+// into the next of NS accumulators in tensor memory and O += P.V, whichever
+// is ready; warps 4-11 (two threads a row, 64 keys each) turn S into P =
+// 2^(c S - m): P is packed into the type and written back over S, from where
+// the second product reads it as its A operand, so it never passes through
+// shared memory. A ring slot holds 8-key groups of [Hd/64][8 keys][128 B], so
+// any page size that is a multiple of 8 gives one layout (group stride Hd/64
+// KB) and the two halves of a tile in neighbouring slots are one operand.
 //
 // The running max is kept until it grows by more than 2^8 (P <= 256 then; O
 // and l use the same max, so O / l is exact for any); the two threads of a
@@ -34,7 +34,7 @@
 // freed pages may hold anything). In tiles that cross a mask edge V rows that
 // no row sees are zeroed, and a value that is not finite, in a row that some
 // see, is taken out of the product and added to their outputs alone: 0 * inf
-// would be NaN for the others.
+// would be NaN for the others (warp 3, before the product may read the slot).
 //
 // Every mbarrier wait is bounded; on give-up the CTA sets the error word,
 // drains, frees its tensor memory and leaves.
@@ -58,8 +58,7 @@ using namespace tc;
 
 constexpr int kM = 128;          // query rows of an item
 constexpr int kN = 128;          // keys of a unit
-constexpr int kSlotKeys = 64;    // keys of a ring slot
-constexpr int kPtThreads = 384;  // warps: 0 TMA, 1 MMA, 4-11 softmax
+constexpr int kPtThreads = 384;  // warps: 0 Q and K loads, 1 MMA, 2 V loads, 3 masked V, 4-11 softmax
 constexpr int kSoftThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 of the growth of a row's max that is let pass
@@ -70,12 +69,21 @@ struct Shape {
     static constexpr int ATOMS = HD / 64;
     static constexpr int NS = HD == 256 ? 2 : 3;  // S accumulators: NS * 128 + HD <= 512 columns
     static constexpr int GROUP = ATOMS * 1024;    // bytes of 8 keys
-    static constexpr int SLOT = 8 * GROUP;
-    static constexpr int NSLOT = HD == 256 ? 5 : (HD == 128 ? 12 : 20);
+    static constexpr int HALVES = HD == 256 ? 2 : 1;  // ring slots of a 128-key tile
+    static constexpr int KEYS = kN / HALVES;          // keys of a slot
+    static constexpr int SLOT = KEYS / 8 * GROUP;
+    static constexpr int NSLOT = HD == 256 ? 5 : (HD == 128 ? 6 : 10);
+    // Warp 0's notes on items and units, a ring. It writes note j with K(j - 1)
+    // in the ring, so K(j - 1 - T) has been read (T tiles fit the ring), which
+    // waited for the product j - 1 - T - NS: entries up to there are free
+    // (Hd 256, whose odd ring mixes K and V: up to j - 4). Warp 3, idle where
+    // nothing is masked, hands its entries back.
+    static constexpr int NOTES = HD == 64 ? 16 : 8;
+    static_assert(HD == 256 || NOTES >= NSLOT / 2 + NS + 1, "notes outlive their readers");
     static constexpr int Q_BLOCK = kM * 128;
     static constexpr int Q_BYTES = ATOMS * Q_BLOCK;
     static constexpr uint32_t O_COL = NS * kN;
-    static constexpr size_t SMEM = size_t(Q_BYTES) + size_t(NSLOT) * SLOT + 1024;
+    static constexpr size_t SMEM = size_t(Q_BYTES) + size_t(NSLOT) * SLOT;  // (1024-byte aligned, behind the static part)
 };
 static_assert(Shape<64>::NSLOT * Shape<64>::SLOT >= (kMaxRequests + 1) * 8, "the plan's sums fit the ring");
 
@@ -92,6 +100,7 @@ struct TcArgs {
     int tpt;        // tokens of an item: 128 / group size
     int group;      // query heads of a KV head
     int box_groups; // 8-key groups of a TMA box
+    uint64_t ps_inv;  // ceil(2^64 / page size)
     int rows_cap;   // rows of a scratch slot
     float c;        // scale * log2(e)
     int64_t groups; // 8-row groups of the pages (past the end: zero fill)
@@ -100,33 +109,34 @@ struct TcArgs {
     Cut* cuts;      // [CTAs]
 };
 
+// All in tokens, keys and tiles (every length is below 2^31).
 struct Item {
-    int r, h, mt;
-    int64_t tok0;  // first token row
-    int ntok;
-    int64_t pos0;          // position of its first token
-    int64_t lo, hi, sink;  // keys that some row sees: [0, sink) and [lo, hi)
-    int64_t len;
+    int r, h;
+    int tok0, ntok;    // token rows
+    int pos0;          // position of the first one
+    int len;           // keys of the request
+    int lo, hi, sink;  // keys that some row sees: [0, sink) and [lo, hi)
     int t_lo, ns, units;  // tiles [0, ns) and from t_lo on
     int u0, u1;           // this CTA's share
     int64_t start;        // the item's first unit in the step's order
 };
 
-__device__ __forceinline__ void item_span(const TcArgs& a, const Request& rq, int mt, Item& it) {
+// (Not inlined: the roles' loops are long, and the instruction cache is what they share.)
+__device__ __noinline__ void item_span(const TcArgs& a, const Request& rq, int mt, Item& it) {
     const PagedAttention& p = a.p;
     const int64_t i0 = int64_t(mt) * a.tpt;
-    it.mt = mt;
-    it.tok0 = rq.t0 + i0;
+    it.tok0 = int(rq.t0 + i0);
     it.ntok = int(rq.n - i0 < a.tpt ? rq.n - i0 : a.tpt);
-    it.pos0 = rq.len - rq.n + i0;
-    it.len = rq.len;
-    const Span first = visible(p, rq, it.pos0), last = visible(p, rq, it.pos0 + it.ntok - 1);
-    it.lo = first.lo;
-    it.hi = last.hi;
-    it.sink = last.sink;
-    it.t_lo = int(it.lo / kN);
-    const int t_hi = int((it.hi + kN - 1) / kN);
-    int ns = int((it.sink + kN - 1) / kN);
+    const int64_t pos0 = rq.len - rq.n + i0;
+    it.pos0 = int(pos0);
+    it.len = int(rq.len);
+    const Span first = visible(p, rq, pos0), last = visible(p, rq, pos0 + it.ntok - 1);
+    it.lo = int(first.lo);
+    it.hi = int(last.hi);
+    it.sink = int(last.sink);
+    it.t_lo = it.lo / kN;
+    const int t_hi = int((last.hi + kN - 1) / kN);
+    const int ns = int((last.sink + kN - 1) / kN);
     it.ns = ns < it.t_lo ? ns : it.t_lo;
     const int u = it.ns + (t_hi > it.t_lo ? t_hi - it.t_lo : 0);
     it.units = u > 1 ? u : 1;  // (rows without a key are written too)
@@ -137,7 +147,7 @@ struct Start {
     int64_t unit, left;
 };
 
-// The CTA's items in order; every role walks them by itself.
+// The CTA's items in order (walked by the load warp, which tells the others).
 struct Walk {
     const TcArgs& a;
     Request rq;
@@ -150,9 +160,9 @@ struct Walk {
     }
     __device__ __forceinline__ void load() {
         rq = request(a.p, r);
-        ntiles = int((rq.n + a.tpt - 1) / a.tpt);
+        ntiles = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
     }
-    __device__ __forceinline__ bool next(Item& it) {
+    __device__ __noinline__ bool next(Item& it) {
         if (left <= 0) return false;
         item_span(a, rq, mt, it);
         it.r = r;
@@ -185,19 +195,56 @@ struct Walk {
 
 __device__ __forceinline__ int tile_of(const Item& it, int u) { return u < it.ns ? u : it.t_lo + (u - it.ns); }
 
-// Every row of the item sees every key of the tile at key0.
-__device__ __forceinline__ bool tile_open(const TcArgs& a, const Item& it, int64_t key0) {
+// Every row of the item sees every one of the `keys` keys from key0 on.
+__device__ __forceinline__ bool keys_open(const TcArgs& a, const Item& it, int64_t key0, int keys) {
     const PagedAttention& p = a.p;
-    const int64_t end = p.mask_kind == 2 ? it.len : (it.pos0 + 1 < it.len ? it.pos0 + 1 : it.len);
-    if (key0 + kN > end) return false;
+    const int64_t end = p.mask_kind == 2 ? it.len : (int64_t(it.pos0) + 1 < it.len ? int64_t(it.pos0) + 1 : it.len);
+    if (key0 + keys > end) return false;
     if (p.mask_kind != 1) return true;
-    return key0 >= it.pos0 + it.ntok - 1 - p.window + 1 || key0 + kN <= p.sinks;
+    return key0 >= int64_t(it.pos0) + it.ntok - p.window || key0 + keys <= p.sinks;
 }
+// Some row of the item sees one of them.
+__device__ __forceinline__ bool keys_seen(const Item& it, int64_t key0, int keys) {
+    return key0 < it.hi && (key0 + keys > it.lo || key0 < it.sink);
+}
+// The V rows of a slot of `keys` keys need a look before the product reads them.
+__device__ __forceinline__ bool guarded(const TcArgs& a, const Item& it, int64_t key0, int keys) {
+    return keys_seen(it, key0, keys) && !keys_open(a, it, key0, keys);
+}
+
+// What warp 0 says of a unit.
+enum : int { kFirst = 1, kLast = 2, kLook = 4 };  // first / last of its item here; kLook << h: half h is guarded
+struct Unit {
+    int flags;
+    int group[16];  // of each box: its first 8-row group of the pages, past the last one for zeros
+};
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// 64 consecutive fp32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, float2* v) {
+    tmem_ld32(addr, reinterpret_cast<float*>(v));
+    tmem_ld32(addr + 32, reinterpret_cast<float*>(v) + 32);
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
@@ -227,24 +274,21 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t stride) {
     return (smem_desc_sw128_mn(saddr, 1024) & ~(uint64_t(0x3fff) << 32)) | (uint64_t(stride >> 4) << 32);
 }
 
-// Warp-uniform bounded wait (seconds of polling); false once any role gave up.
-__device__ __forceinline__ bool wait_bar(uint64_t& bar, uint32_t parity, int lane, volatile int& abort) {
-    int ok = 0;
-    if (lane == 0) {
-        const uint32_t b = smem_u32(&bar);
-        for (uint32_t i = 0; i < (1u << 26); ++i) {
-            if (mbar_test_wait(b, parity)) {
-                ok = 1;
-                break;
-            }
-            if ((i & 1023u) == 1023u && abort) break;
-        }
-        if (!ok && !abort) {
-            atomicOr(&g_pt_error_word, 1u);
-            abort = 1;
-        }
+// Warp-uniform bounded wait (20000 suspended tries of at most 0.1 ms); false
+// once any role gave up.
+__device__ __noinline__ bool wait_long(uint32_t b, uint32_t parity, volatile int* abort) {
+    for (int i = 0; i < 20000; ++i) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
+        if (__any_sync(0xffffffffu, *abort != 0)) return false;
     }
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    if ((threadIdx.x & 31) == 0) atomicOr(&g_pt_error_word, 1u);
+    *abort = 1;
+    return false;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t& bar, uint32_t parity, volatile int& abort) {
+    const uint32_t b = smem_u32(&bar);
+    if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
+    return wait_long(b, parity, &abort);
 }
 
 // Barrier `id` over the softmax threads; true where any of them says so.
@@ -261,18 +305,51 @@ __device__ __forceinline__ bool soft_any(int id, bool mine) {
     return any != 0;
 }
 
-// A half word pair that holds an infinity or a NaN.
+// Exponent fields of two 16-bit values: bit 15 of a half is set in the result where its value is not finite.
 template <class T>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-    constexpr uint32_t e = T::code == TBF16::code ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+    constexpr uint32_t e = T::code == TBF16::code ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t one = T::code == TBF16::code ? 0x00800080u : 0x04000400u;
+    return (w & e) + one;
 }
 template <class T>
 __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
-    constexpr uint32_t e = T::code == TBF16::code ? 0x7f80u : 0x7c00u;
-    if ((w & e) == e) w &= 0xffff0000u;
-    if (((w >> 16) & e) == e) w &= 0x0000ffffu;
-    return w;
+    const uint32_t bad = not_finite2<T>(w) & 0x80008000u;
+    return w & ~((bad >> 15) * 0xffffu);
+}
+
+// The product left out V values that are not finite, in slots where some row does not see some key: adds them to the
+// rows that see them (an infinity or a NaN outweighs any weight). O's columns [w Hd / 2, (w + 1) Hd / 2) are at `o_addr`.
+template <int HD, class T>
+__device__ __noinline__ void add_not_finite(const TcArgs& a, const Item& it, const Span& v, int w, uint32_t o_addr) {
+    const PagedAttention& p = a.p;
+    constexpr int KEYS = Shape<HD>::KEYS;
+#pragma unroll 1
+    for (int x = it.u0; x < it.u1; ++x) {
+        const int64_t key0 = int64_t(tile_of(it, x)) * kN;
+#pragma unroll 1
+        for (int64_t key = key0; key < key0 + kN; ++key) {
+            if (!keys_seen(it, key, 1) || !guarded(a, it, key & ~int64_t(KEYS - 1), KEYS)) continue;
+            const int32_t page = p.table[int64_t(it.r) * p.W + key / p.ps];
+            if (page < 0 || page >= p.P) continue;
+            const bool sees = (key >= v.lo && key < v.hi) || key < v.sink;
+            const int64_t vrow = ((int64_t(page) * p.Nkv + it.h) * p.ps + key % p.ps) * HD + w * (HD / 2);
+#pragma unroll 1
+            for (int cc = 0; cc < HD / 64; ++cc) {
+                const float mine = Elem<T>::load(p.v_pages, vrow + cc * 32 + (threadIdx.x & 31));
+                if (!__any_sync(0xffffffffu, !(fabsf(mine) <= 3.4e38f))) continue;
+                float o[32];
+                tmem_ld32(o_addr + cc * 32, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float y = Elem<T>::load(p.v_pages, vrow + cc * 32 + e);
+                    if (sees && !(fabsf(y) <= 3.4e38f)) o[e] += y;
+                }
+                tmem_st32(o_addr + cc * 32, o);
+                tmem_wait_st();
+            }
+        }
+    }
 }
 
 template <int HD, class T>
@@ -281,20 +358,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                               const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                               const __grid_constant__ TcArgs a) {
     using S = Shape<HD>;
-    constexpr int NS = S::NS, NSLOT = S::NSLOT, ATOMS = S::ATOMS;
+    constexpr int NS = S::NS, NSLOT = S::NSLOT, ATOMS = S::ATOMS, kNotes = S::NOTES;
     constexpr bool BF = T::code == TBF16::code;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t q_full, q_empty, full[NSLOT], empty[NSLOT], s_full[NS], p_full[NS], pv_done[NS], o_free;
+    __shared__ __align__(8) uint64_t item_full[kNotes], unit_full[kNotes], unit_free[kNotes], look[kNotes], q_full, q_empty,
+        full[NSLOT], empty[NSLOT], s_full[NS], p_full[NS], pv_done[NS], o_free;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ Start s_start;
     __shared__ long long s_scan[kPtThreads / 32];
     __shared__ float s_mx[2][kM];  // a row's two maxima, at an item's end its two sums
-    __shared__ uint32_t s_poison[3][4];
+    __shared__ Item s_item[kNotes];
+    __shared__ volatile int s_poison[kNotes];  // an item has V values that are not finite in a tile with masked keys
+    __shared__ Unit s_unit[kNotes];
 
     pdl_launch_dependents();
-    unsigned char* sq =
-        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* sq = smem_raw;
+    if (smem_u32(sq) & 1023u) {  // (the swizzle's pattern repeats every 1024 bytes of address)
+        if (threadIdx.x == 0) atomicOr(&g_pt_error_word, 1u);
+        return;
+    }
     unsigned char* ring = sq + S::Q_BYTES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedAttention& p = a.p;
@@ -302,6 +385,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     if (tid == 0) {
         mbar_init(smem_u32(&q_full), 1);
         mbar_init(smem_u32(&q_empty), 1);
+        for (int i = 0; i < kNotes; ++i) {
+            mbar_init(smem_u32(&item_full[i]), 1);
+            mbar_init(smem_u32(&unit_full[i]), 1);
+            mbar_init(smem_u32(&unit_free[i]), 1);
+            mbar_init(smem_u32(&look[i]), 1);
+        }
         for (int i = 0; i < NSLOT; ++i) {
             mbar_init(smem_u32(&full[i]), 1);
             mbar_init(smem_u32(&empty[i]), 1);
@@ -315,7 +404,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         s_abort = 0;
         mbar_fence_init();
     }
-    if (tid < 12) (&s_poison[0][0])[tid] = 0;
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), kTmem);
     pdl_wait();
 
@@ -323,7 +411,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     long long* cum = reinterpret_cast<long long*>(ring);  // [R + 1], before any copy uses the ring
     auto head_units = [&](const Request& rq, int from, int step) {
         long long u = 0;
-        const int nt = int((rq.n + a.tpt - 1) / a.tpt);
+        const int nt = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
         Item it;
         for (int mt = from; mt < nt; mt += step) {
             item_span(a, rq, mt, it);
@@ -385,7 +473,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             rem -= s.h * per_head;
             // the item: 32 tiles at a time
             const Request rq = request(p, lo);
-            const int nt = int((rq.n + a.tpt - 1) / a.tpt);
+            const int nt = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
             for (int mt0 = 0; mt0 < nt; mt0 += 32) {
                 Item it;
                 it.units = 0;
@@ -415,166 +503,212 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t tmem = s_tmem;
     const Start start = s_start;
 
-    if (warp == 0) {
-        // ---- loads ----
-        Walk walk(a, start);
-        Item it, prev;
-        const uint32_t ring_a = smem_u32(ring);
-        const int boxes = 8 / a.box_groups;
-        const uint32_t box_bytes = uint32_t(a.box_groups * S::GROUP);
-        const uint32_t ps = uint32_t(p.ps);
+    const int n = int(start.left);  // units of this CTA
+    constexpr int H = S::HALVES;    // ring positions of a K or V tile, from k_pos / v_pos on
+    auto k_pos = [&](int j) { return j == 0 ? 0 : (2 * j - 1) * H; };
+    auto v_pos = [&](int j) { return (j == n - 1 ? 2 * n - 1 : 2 * j + 2) * H; };
+    // Item k of this CTA, once warp 0 has published it.
+    auto item = [&](int k, Item& it) {
+        if (!wait_bar(item_full[k % kNotes], uint32_t(k / kNotes) & 1u, s_abort)) return false;
+        it = s_item[k % kNotes];
+        return true;
+    };
+    const int boxes = kN / 8 / a.box_groups;  // TMA boxes of a tile
+    // Box b of H-th part h, its share of the tile: issued one by one by lane 0.
+    auto put = [&](const int* group, int pos, uint64_t* const* bars, const CUtensorMap* map) {
         bool ok = true;
-        int issued = 0;  // ring positions issued
-        // This lane's box of the 64 keys at key0: its first group, or past the end for keys that no row sees.
-        auto group_of = [&](const Item& t, int64_t key0) -> int {
-            int64_t g = a.groups;
-            const int64_t k0 = key0 + lane * a.box_groups * 8;
-            if (lane < boxes && k0 < t.hi && (k0 + a.box_groups * 8 > t.lo || k0 < t.sink)) {
-                const uint32_t k = uint32_t(k0);
-                const int32_t page = p.table[int64_t(t.r) * p.W + k / ps];
-                if (page >= 0 && page < p.P) g = ((int64_t(page) * p.Nkv + t.h) * p.ps + k % ps) / 8;
-                else atomicOr(&g_pt_error_word, 32u);
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int q = pos + h, slot = q % NSLOT;
+            ok = wait_bar(empty[slot], (uint32_t(q / NSLOT) & 1u) ^ 1u, s_abort);
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t bar = smem_u32(bars[h] ? bars[h] : &full[slot]);
+                const uint32_t dst = smem_u32(ring) + slot * S::SLOT;
+                const int per = boxes / H;
+                mbar_expect_tx(bar, S::SLOT);
+                for (int b = 0; b < per; ++b)
+                    tma_load_4d(dst + b * a.box_groups * S::GROUP, map, 0, 0, 0, group[h * per + b], bar);
             }
-            return int(g);
+        }
+        __syncwarp();
+        return ok;
+    };
+
+    if (warp == 0) {
+        // ---- items, pages, Q and K ----
+        Walk walk(a, start);
+        bool ok = true;
+        const int box_keys = a.box_groups * 8;
+        const int per_fill = 32 / boxes;  // units whose boxes one look at the table covers
+        const int my_unit = lane / boxes, my_box = lane % boxes;
+        // The page of this lane's box, of unit u + my_unit (-1: no row sees a key of it). Read ahead: the table's
+        // latency is longer than a tile's loads take to issue.
+        auto page_of = [&](const Item& t, int u) {
+            if (u + my_unit >= t.u1) return -1;
+            const int64_t k0 = int64_t(tile_of(t, u + my_unit)) * kN + my_box * box_keys;
+            if (!keys_seen(t, k0, box_keys)) return -1;
+            const int32_t page = p.table[int64_t(t.r) * p.W + int64_t(__umul64hi(uint64_t(k0), a.ps_inv))];
+            return page >= 0 ? page : 0x7fffffff;
         };
-        auto put = [&](const Item& t, int u, int pos, const CUtensorMap* map) {
-#pragma unroll 1
-            for (int half = 0; half < 2 && ok; ++half) {
-                const int64_t key0 = int64_t(tile_of(t, u)) * kN + half * kSlotKeys;
-                const int g = group_of(t, key0);
-                const int q = pos + half, slot = q % NSLOT;
-                ok = wait_bar(empty[slot], (uint32_t(q / NSLOT) & 1u) ^ 1u, lane, s_abort);
-                if (!ok) return;
-                const uint32_t bar = smem_u32(&full[slot]);
-                if (lane == 0) mbar_expect_tx(bar, S::SLOT);
+        auto group_of = [&](const Item& t, int u, int page) {
+            if (page < 0) return int(a.groups);
+            if (page >= p.P) {
+                atomicOr(&g_pt_error_word, 32u);
+                return int(a.groups);
+            }
+            const uint32_t k = uint32_t(tile_of(t, u + my_unit) * kN + my_box * box_keys);
+            const uint32_t off = k - uint32_t(__umul64hi(uint64_t(k), a.ps_inv)) * uint32_t(p.ps);
+            return int((uint32_t(page) * uint32_t(p.Nkv) + uint32_t(t.h)) * (uint32_t(p.ps) / 8) + off / 8);
+        };
+        Item it, nx;  // the item at hand, and the one of the next look
+        int items = 0, nu = 0, page = -1, j = 0;
+        bool more = n > 0 && walk.next(nx);
+        if (more) {
+            nu = nx.u0;
+            page = page_of(nx, nu);
+        }
+        while (more && ok) {
+            it = nx;
+            const int u_first = nu;
+            const int g = group_of(it, u_first, page);
+            const int u_end = u_first + per_fill < it.u1 ? u_first + per_fill : it.u1;
+            if (u_end < it.u1) {
+                nu = u_end;
+            } else {
+                more = walk.next(nx);
+                nu = nx.u0;
+            }
+            if (more) page = page_of(nx, nu);
+            for (int u = u_first; u < u_end && ok; ++u, ++j) {
+                Unit& note = s_unit[j % kNotes];
+                ok = wait_bar(unit_free[j % kNotes], (uint32_t(j / kNotes) & 1u) ^ 1u, s_abort);
+                if (!ok) break;
+                if (my_unit == u - u_first) note.group[my_box] = g;
                 __syncwarp();
-                if (lane < boxes) tma_load_4d(ring_a + slot * S::SLOT + lane * box_bytes, map, 0, 0, 0, g, bar);
-                issued = q + 1;
-            }
-        };
-        int j = 0, items = 0, prev_u = -1;
-        bool q_pending = false;
-        while (ok && walk.next(it)) {
-            for (int u = it.u0; u < it.u1 && ok; ++u, ++j) {
+                if (lane == 0) {
+                    int flags = (u == it.u0 ? kFirst : 0) | (u == it.u1 - 1 ? kLast : 0);
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                        if (guarded(a, it, int64_t(tile_of(it, u)) * kN + h * S::KEYS, S::KEYS)) flags |= kLook << h;
+                    note.flags = flags;
+                    if (u == it.u0) {
+                        s_poison[items % kNotes] = 0;
+                        s_item[items % kNotes] = it;
+                        mbar_arrive(smem_u32(&item_full[items % kNotes]));
+                    }
+                    mbar_arrive(smem_u32(&unit_full[j % kNotes]));
+                }
+                __syncwarp();
                 if (u == it.u0) {
-                    if (j > 0) put(prev, prev_u, 4 * j - 2, &map_v);
-                    if (!ok) break;
-                    ok = wait_bar(q_empty, (uint32_t(items) & 1u) ^ 1u, lane, s_abort);
+                    ok = wait_bar(q_empty, (uint32_t(items) & 1u) ^ 1u, s_abort);
                     if (!ok) break;
                     if (lane == 0) {
                         const bool one = it.ntok == 1;
-                        const uint32_t rows = uint32_t(one ? a.group : a.group * a.tpt);
-                        mbar_expect_tx(smem_u32(&q_full), rows * 128 * ATOMS);
-#pragma unroll
+                        mbar_expect_tx(smem_u32(&q_full), uint32_t(one ? a.group : a.group * a.tpt) * 128 * ATOMS);
                         for (int at = 0; at < ATOMS; ++at)
-                            tma_load_4d(smem_u32(sq + at * S::Q_BLOCK), one ? &map_q1 : &map_q, 0, it.h * a.group,
-                                        int(it.tok0), at, smem_u32(&q_full));
+                            tma_load_4d(smem_u32(sq + at * S::Q_BLOCK), one ? &map_q1 : &map_q, 0, it.h * a.group, it.tok0, at,
+                                        smem_u32(&q_full));
                     }
                     __syncwarp();
-                    q_pending = true;
                     ++items;
-                    put(it, u, 4 * j, &map_k);
-                } else {
-                    put(it, u, 4 * j - 2, &map_k);
-                    put(prev, prev_u, 4 * j, &map_v);
                 }
-                prev = it;
-                prev_u = u;
+                uint64_t* const none[2] = {nullptr, nullptr};
+                ok = put(note.group, k_pos(j), none, &map_k);
             }
         }
-        if (ok && j > 0) put(prev, prev_u, 4 * j - 2, &map_v);
-        if (!ok) {
-            s_abort = 1;
-            // leave no copy in flight
-            if (lane == 0) {
-                if (q_pending) mbar_wait(smem_u32(&q_full), uint32_t(items - 1) & 1u, &g_pt_error_word);
-                for (int q = issued - NSLOT < 0 ? 0 : issued - NSLOT; q < issued; ++q)
-                    mbar_wait(smem_u32(&full[q % NSLOT]), uint32_t(q / NSLOT) & 1u, &g_pt_error_word);
-            }
+        if (!ok) s_abort = 1;
+    } else if (warp == 2) {
+        // ---- V ----
+        bool ok = true;
+        int looks = 0;
+        for (int j = 0; j < n && ok; ++j) {
+            ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
+            if (!ok) break;
+            const Unit& note = s_unit[j % kNotes];
+            uint64_t* to[2] = {nullptr, nullptr};
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                if (note.flags & (kLook << h)) to[h] = &look[looks++ % kNotes];
+            ok = put(note.group, v_pos(j), to, &map_v);
         }
+        if (!ok) s_abort = 1;
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && n > 0) {
             // ---- MMA issue ----
-            constexpr uint32_t idesc_s = make_idesc(BF, kM, kN, false), idesc_h = make_idesc(BF, kM, kSlotKeys, false);
+            constexpr uint32_t idesc_s = make_idesc(BF, kM, kN, false), idesc_h = make_idesc(BF, kM, kN / 2, false);
             constexpr uint32_t idesc_o = make_idesc(BF, kM, HD, true);
             const uint32_t q_base = smem_u32(sq), ring_a = smem_u32(ring);
             auto is_full = [&](int q) {
                 return mbar_test_wait(smem_u32(&full[q % NSLOT]), uint32_t(q / NSLOT) & 1u);
             };
-            Walk walk_s(a, start), walk_p(a, start);
-            Item is, ip;
-            const int n = int(start.left);
-            int ns = 0, np = 0;
-            int us = 0, up = 0, items_s = 0, items_p = 0;
+            int ns = 0, np = 0;  // next tile of S, of O
+            int ks = 0, kp = 0;  // their items
+            int fs = 0;          // the notes on tile ns (0: not read yet)
             bool ok = true;
-            if (n > 0) {
-                walk_s.next(is);
-                walk_p.next(ip);
-                us = is.u0;
-                up = ip.u0;
-            }
             uint32_t idle = 0;
             while (np < n && !s_abort) {
                 bool progressed = false;
                 if (ns < n && ns < np + NS) {
                     const int buf = ns % NS;
-                    const bool first = us == is.u0;
-                    const int q0 = first ? 4 * ns : 4 * ns - 2, q1 = q0 + 1;
-                    if ((ns < NS || mbar_test_wait(smem_u32(&pv_done[buf]), uint32_t(ns / NS - 1) & 1u)) &&
-                        (!first || mbar_test_wait(smem_u32(&q_full), uint32_t(items_s) & 1u)) && is_full(q0) && is_full(q1)) {
+                    const int q0 = k_pos(ns), q1 = q0 + H - 1;
+                    if (fs == 0 && mbar_test_wait(smem_u32(&unit_full[ns % kNotes]), uint32_t(ns / kNotes) & 1u))
+                        fs = s_unit[ns % kNotes].flags | 256;
+                    if (fs && (ns < NS || mbar_test_wait(smem_u32(&pv_done[buf]), uint32_t(ns / NS - 1) & 1u)) &&
+                        (!(fs & kFirst) || mbar_test_wait(smem_u32(&q_full), uint32_t(ks) & 1u)) && is_full(q0) &&
+                        (H == 1 || is_full(q1))) {
                         tc_fence_after();
                         const int s0 = q0 % NSLOT, s1 = q1 % NSLOT;
                         const uint32_t k0 = ring_a + s0 * S::SLOT, k1 = ring_a + s1 * S::SLOT;
                         const uint32_t d = tmem + uint32_t(buf * kN);
-                        if (s1 == s0 + 1) {
+                        // one N = 128 product, or two of 64 where the tile wraps round the ring
+                        const bool one = H == 1 || s1 == s0 + 1;
+#pragma unroll 1
+                        for (int h = 0; h < (one ? 1 : 2); ++h) {
+                            uint64_t da = smem_desc_sw128(q_base), db = desc_k(h ? k1 : k0, S::GROUP);
+                            const uint32_t to = d + uint32_t(h * (kN / 2)), idesc = one ? idesc_s : idesc_h;
+#pragma unroll 1
+                            for (int at = 0; at < ATOMS; ++at) {
 #pragma unroll
-                            for (int kk = 0; kk < HD / 16; ++kk)
-                                tc_mma(d, smem_desc_sw128(q_base + (kk >> 2) * S::Q_BLOCK + (kk & 3) * 32),
-                                       desc_k(k0 + (kk >> 2) * 1024 + (kk & 3) * 32, S::GROUP), idesc_s, kk > 0 ? 1u : 0u);
-                        } else {  // the tile wraps round the ring: two halves
-#pragma unroll
-                            for (int kk = 0; kk < HD / 16; ++kk)
-                                tc_mma(d, smem_desc_sw128(q_base + (kk >> 2) * S::Q_BLOCK + (kk & 3) * 32),
-                                       desc_k(k0 + (kk >> 2) * 1024 + (kk & 3) * 32, S::GROUP), idesc_h, kk > 0 ? 1u : 0u);
-#pragma unroll
-                            for (int kk = 0; kk < HD / 16; ++kk)
-                                tc_mma(d + kSlotKeys, smem_desc_sw128(q_base + (kk >> 2) * S::Q_BLOCK + (kk & 3) * 32),
-                                       desc_k(k1 + (kk >> 2) * 1024 + (kk & 3) * 32, S::GROUP), idesc_h, kk > 0 ? 1u : 0u);
+                                for (int kk = 0; kk < 4; ++kk) tc_mma(to, da + 2 * kk, db + 2 * kk, idesc, (at | kk) ? 1u : 0u);
+                                da += S::Q_BLOCK >> 4;
+                                db += 1024 >> 4;
+                            }
                         }
                         tc_commit(smem_u32(&empty[s0]));
-                        tc_commit(smem_u32(&empty[s1]));
+                        if (H > 1) tc_commit(smem_u32(&empty[s1]));
                         tc_commit(smem_u32(&s_full[buf]));
-                        if (us == is.u1 - 1) tc_commit(smem_u32(&q_empty));
-                        if (++us == is.u1) {
-                            ++items_s;
-                            if (walk_s.next(is)) us = is.u0;
-                        }
+                        if (fs & kFirst) ++ks;
+                        if (fs & kLast) tc_commit(smem_u32(&q_empty));
+                        fs = 0;
                         ++ns;
                         progressed = true;
                     }
                 }
                 if (np < ns) {
                     const int buf = np % NS;
-                    const bool first = up == ip.u0, last = up == ip.u1 - 1;
-                    const int q0 = last ? 4 * np + 2 : 4 * np + 4, q1 = q0 + 1;
-                    if (mbar_test_wait(smem_u32(&p_full[buf]), uint32_t(np / NS) & 1u) && is_full(q0) && is_full(q1) &&
-                        (!first || items_p == 0 || mbar_test_wait(smem_u32(&o_free), uint32_t(items_p - 1) & 1u))) {
+                    const int q0 = v_pos(np), q1 = q0 + H - 1;
+                    const int fp = s_unit[np % kNotes].flags;
+                    const bool first = fp & kFirst;
+                    if (mbar_test_wait(smem_u32(&p_full[buf]), uint32_t(np / NS) & 1u) && is_full(q0) &&
+                        (H == 1 || is_full(q1)) &&
+                        (!first || kp == 0 || mbar_test_wait(smem_u32(&o_free), uint32_t(kp - 1) & 1u))) {
                         tc_fence_after();
                         const int s0 = q0 % NSLOT, s1 = q1 % NSLOT;
                         const uint32_t pa = tmem + uint32_t(buf * kN);
+#pragma unroll 1
+                        for (int h = 0; h < 2; ++h) {  // 64 keys each
+                            const uint32_t v = ring_a + (H == 1 ? s0 * S::SLOT + h * (S::SLOT / 2) : (h ? s1 : s0) * S::SLOT);
+                            const uint64_t db = desc_mn(v, S::GROUP);
 #pragma unroll
-                        for (int kk = 0; kk < kN / 16; ++kk) {
-                            const uint32_t v = ring_a + (kk < 4 ? s0 : s1) * S::SLOT + (kk & 3) * 2 * S::GROUP;
-                            tc_mma_ts(tmem + S::O_COL, pa + kk * 8, desc_mn(v, S::GROUP), idesc_o,
-                                      (!first || kk > 0) ? 1u : 0u);
+                            for (int kk = 0; kk < 4; ++kk)
+                                tc_mma_ts(tmem + S::O_COL, pa + (4 * h + kk) * 8, db + uint64_t(kk * (2 * S::GROUP >> 4)), idesc_o,
+                                          (!first || h > 0 || kk > 0) ? 1u : 0u);
                         }
                         tc_commit(smem_u32(&empty[s0]));
-                        tc_commit(smem_u32(&empty[s1]));
+                        if (H > 1) tc_commit(smem_u32(&empty[s1]));
                         tc_commit(smem_u32(&pv_done[buf]));
-                        if (++up == ip.u1) {
-                            ++items_p;
-                            if (walk_p.next(ip)) up = ip.u0;
-                        }
+                        if (first) ++kp;
                         ++np;
                         progressed = true;
                     }
@@ -589,6 +723,67 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             }
             if (!ok) s_abort = 1;
         }
+    } else if (warp == 3) {
+        // ---- V of slots with masked keys ----
+        Item it;
+        bool ok = true;
+        int looks = 0;
+        for (int j = 0, k = -1; j < n && ok; ++j) {
+            ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
+            if (!ok) break;
+            const int flags = s_unit[j % kNotes].flags;
+            if (flags & kFirst) {
+                ok = item(++k, it);
+                if (!ok) break;
+                it.units = it.u0;  // (here: the unit at hand)
+            } else {
+                ++it.units;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&unit_free[j % kNotes]));
+            for (int h = 0; h < H && ok; ++h) {
+                if (!(flags & (kLook << h))) continue;
+                const int64_t key0 = int64_t(tile_of(it, it.units)) * kN + h * S::KEYS;
+                const int slot = (v_pos(j) + h) % NSLOT;
+                ok = wait_bar(look[looks % kNotes], uint32_t(looks / kNotes) & 1u, s_abort);
+                ++looks;
+                if (!ok) break;
+                bool bad = false;
+#pragma unroll 1
+                for (int kk = lane; kk < S::KEYS; kk += 32) {
+                    const int64_t key = key0 + kk;
+                    if (keys_open(a, it, key, 1)) continue;  // (no row's product has a zero for it)
+                    const bool seen = keys_seen(it, key, 1);
+                    unsigned char* base = ring + slot * S::SLOT + (kk >> 3) * S::GROUP + (kk & 7) * 128;
+                    uint32_t any = 0;
+                    if (seen) {
+#pragma unroll 8
+                        for (int i = 0; i < ATOMS * 8; ++i) {
+                            const uint4 y = *reinterpret_cast<const uint4*>(base + (i >> 3) * 1024 + ((i + kk) & 7) * 16);
+                            any |= not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w);
+                        }
+                    }
+                    if (seen && !(any & 0x80008000u)) continue;
+#pragma unroll 8
+                    for (int i = 0; i < ATOMS * 8; ++i) {
+                        uint4* x = reinterpret_cast<uint4*>(base + (i >> 3) * 1024 + ((i + kk) & 7) * 16);
+                        uint4 y = make_uint4(0, 0, 0, 0);
+                        if (seen) {
+                            y = *x;
+                            y = make_uint4(finite_part<T>(y.x), finite_part<T>(y.y), finite_part<T>(y.z), finite_part<T>(y.w));
+                        }
+                        *x = y;
+                    }
+                    bad = bad || seen;
+                }
+                if (bad) s_poison[k % kNotes] = 1;
+                __threadfence_block();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&full[slot]));
+            }
+        }
+        if (!ok) s_abort = 1;
     } else if (warp >= 4) {
         // ---- softmax: row (warp % 4) * 32 + lane, keys [64 w, 64 w + 64) of each tile ----
         const int w = (warp - 4) >> 2;
@@ -597,82 +792,57 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int soft = (warp - 4) * 32 + lane;
         const uint32_t lane_off = uint32_t(quarter * 32) << 16;
         const int ti = row / a.group, gi = row % a.group;
-        Walk walk(a, start);
         Item it;
         bool ok = true;  // (once false, the barriers below are still met, so that no warp is left at one)
         int j = 0;
         Cut cut{0, 0, 0, -1, 0};
-        while (walk.next(it)) {
+        for (int k = 0; j < n; ++k) {
+            if (ok) ok = item(k, it);
+            if (soft_any(2, !ok)) {  // (all leave together)
+                ok = false;
+                break;
+            }
             const int rows = it.ntok * a.group;
             const bool valid = row < rows;
             const bool live = quarter * 32 < rows;  // some row of the warp is there
-            Span v = visible(p, Request{it.tok0, it.ntok, it.len}, it.pos0 + ti);
+            Span v = visible(p, Request{it.tok0, it.ntok, it.len}, int64_t(it.pos0) + ti);
             if (!valid) v = Span{0, 0, 0};
             float m = -INFINITY, l = 0.f;
             for (int u = it.u0; u < it.u1; ++u, ++j) {
                 const int buf = j % NS;
-                const int64_t key0 = int64_t(tile_of(it, u)) * kN;
-                const bool open = tile_open(a, it, key0);
-                if (ok) ok = wait_bar(s_full[buf], uint32_t(j / NS) & 1u, lane, s_abort);
+                const int64_t key0 = int64_t(tile_of(it, u)) * kN + w * 64;  // this thread's 64 keys
+                const bool open = keys_open(a, it, key0, 64);
+                if (ok) ok = wait_bar(s_full[buf], uint32_t(j / NS) & 1u, s_abort);
                 tc_fence_after();
-                float s[64];
+                float2 s[32];
                 float mx = -INFINITY;
                 if (ok && live) {
-                    tmem_ld32(tmem + uint32_t(buf * kN + w * 64) + lane_off, s);
-                    tmem_ld32(tmem + uint32_t(buf * kN + w * 64 + 32) + lane_off, s + 32);
+                    tmem_ld64(tmem + uint32_t(buf * kN + w * 64) + lane_off, s);
                     if (!open) {
-                        const int64_t k0 = key0 + w * 64;
-                        auto rel = [&](int64_t x) { return int(x - k0 < 0 ? 0 : (x - k0 > 64 ? 64 : x - k0)); };
-                        const int lo = rel(v.lo), hi = rel(v.hi), sk = rel(v.sink);
+                        // bit c: this row sees key c of the thread's 64
+                        auto below = [&](int64_t x) {
+                            const int64_t n = x - key0;
+                            return n <= 0 ? uint64_t(0) : (n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1);
+                        };
+                        const uint64_t sees = (below(v.hi) & ~below(v.lo)) | below(v.sink);
+                        const uint32_t bits[2] = {uint32_t(sees), uint32_t(sees >> 32)};
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (!((c >= lo && c < hi) || c < sk)) s[c] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) mx = fmaxf(mx, s[c]);
-                    mx *= a.c;
-                }
-                if (!open) {
-                    // V rows of this tile: what is not finite leaves the product (see the file's comment). The slot's
-                    // barrier is only ever one phase ahead: the product before has to be done first.
-                    if (ok && u > it.u0)
-                        ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, lane, s_abort);
-                    const int key = soft & 127;
-                    const int q = (u == it.u1 - 1 ? 4 * j + 2 : 4 * j + 4) + (key >> 6);
-                    if (ok) ok = wait_bar(full[q % NSLOT], uint32_t(q / NSLOT) & 1u, lane, s_abort);
-                    if (ok) {
-                        const int64_t k = key0 + key;
-                        const bool seen = (k >= it.lo && k < it.hi) || k < it.sink;
-                        unsigned char* base = ring + (q % NSLOT) * S::SLOT + ((key & 63) >> 3) * S::GROUP + (key & 7) * 128;
-                        bool wrote = false, bad = false;
-#pragma unroll 4
-                        for (int i = 0; i < (ATOMS == 1 ? 4 : ATOMS * 4); ++i) {
-                            const int at = ATOMS == 1 ? 0 : w * (ATOMS / 2) + (i >> 3);
-                            const int ch = ATOMS == 1 ? 4 * w + ((i + key) & 3) : ((i + key) & 7);
-                            uint4* x = reinterpret_cast<uint4*>(base + at * 1024 + ch * 16);
-                            const uint4 y = *x;
-                            if (!seen) {
-                                *x = make_uint4(0, 0, 0, 0);
-                                wrote = true;
-                            } else if (not_finite2<T>(y.x) || not_finite2<T>(y.y) || not_finite2<T>(y.z) ||
-                                       not_finite2<T>(y.w)) {
-                                *x = make_uint4(finite_part<T>(y.x), finite_part<T>(y.y), finite_part<T>(y.z),
-                                                finite_part<T>(y.w));
-                                wrote = bad = true;
-                            }
+                        for (int c = 0; c < 32; ++c) {
+                            if (!(bits[c >> 4] & (1u << (2 * (c & 15))))) s[c].x = -INFINITY;
+                            if (!(bits[c >> 4] & (2u << (2 * (c & 15))))) s[c].y = -INFINITY;
                         }
-                        if (bad) atomicOr(&s_poison[j % 3][key >> 5], 1u << (key & 31));
-                        if (wrote) fence_async_smem();
                     }
+                    float m0 = s[0].x, m1 = s[0].y, m2 = s[1].x, m3 = s[1].y;
+#pragma unroll
+                    for (int c = 2; c < 32; c += 2) {
+                        m0 = fmaxf(m0, s[c].x);
+                        m1 = fmaxf(m1, s[c].y);
+                        m2 = fmaxf(m2, s[c + 1].x);
+                        m3 = fmaxf(m3, s[c + 1].y);
+                    }
+                    mx = fmaxf(mx, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.c);
                 }
-                const bool grow = soft_any(1, ok && valid && mx > m + kGrow);
-                if (soft < 4) s_poison[(j + 2) % 3][soft] = 0;  // (last read before this barrier, next set after another)
-                bool poison = false;
-                if (!open) {
-                    const uint32_t* z = s_poison[j % 3];
-                    poison = (z[0] | z[1] | z[2] | z[3]) != 0;
-                }
-                if (grow) {
+                if (soft_any(1, ok && valid && mx > m + kGrow)) {
                     s_mx[w][row] = mx;
                     soft_any(2, false);
                     const float both = fmaxf(s_mx[0][row], s_mx[1][row]);
@@ -684,7 +854,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     }
                     if (ok && u > it.u0 && __any_sync(0xffffffffu, f != 1.f)) {
                         // O was accumulated under the old max
-                        ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, lane, s_abort);
+                        ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, s_abort);
                         tc_fence_after();
                         if (ok) {
                             // (f 0: a row whose keys so far weighed nothing; its O is zero)
@@ -704,56 +874,34 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 }
                 if (ok && live) {
                     const float mu = m == -INFINITY ? 0.f : m;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        s[c] = ex2(fmaf(s[c], a.c, -mu));
-                        sum += s[c];
-                    }
-                    l += sum;
+                    const float2 c2 = make_float2(a.c, a.c), m2 = make_float2(-mu, -mu);
+                    float2 sum0 = make_float2(l, 0.f), sum1 = make_float2(0.f, 0.f);
                     float pk[32];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) pk[c] = __uint_as_float(cvt_pair<T>(s[2 * c], s[2 * c + 1]));
+                    for (int c = 0; c < 32; ++c) {
+                        float2 x = fma2(s[c], c2, m2);
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        if (c & 1) sum1 = add2(sum1, x);
+                        else sum0 = add2(sum0, x);
+                        pk[c] = __uint_as_float(cvt_pair<T>(x.x, x.y));
+                    }
+                    sum0 = add2(sum0, sum1);
+                    l = sum0.x + sum0.y;
                     tmem_st32(tmem + uint32_t(buf * kN + w * 32) + lane_off, pk);
                     tmem_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&p_full[buf]));
-                if (poison && ok) {
-                    // add what is not finite to the rows that see its key, once the product is done
-                    ok = wait_bar(pv_done[buf], uint32_t(j / NS) & 1u, lane, s_abort);
-                    tc_fence_after();
-                    for (int key = 0; key < kN && ok; ++key) {
-                        if (!((s_poison[j % 3][key >> 5] >> (key & 31)) & 1u)) continue;
-                        const int64_t k = key0 + key;
-                        const bool sees = (k >= v.lo && k < v.hi) || k < v.sink;
-                        const int32_t page = p.table[int64_t(it.r) * p.W + k / p.ps];
-                        if (page < 0 || page >= p.P) continue;
-                        const int64_t vrow = ((int64_t(page) * p.Nkv + it.h) * p.ps + k % p.ps) * HD;
-#pragma unroll 1
-                        for (int cc = 0; cc < HD / 64; ++cc) {
-                            float o[32];
-                            const int col = w * (HD / 2) + cc * 32;
-                            const uint32_t at = tmem + S::O_COL + uint32_t(col) + lane_off;
-                            tmem_ld32(at, o);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float x = Elem<T>::load(p.v_pages, vrow + col + e);
-                                if (sees && !(fabsf(x) <= 3.4e38f)) o[e] += x;
-                            }
-                            tmem_st32(at, o);
-                        }
-                        tmem_wait_st();
-                    }
-                    tc_fence_before();
-                }
             }
             // ---- the item's share is summed: O / l, or its piece ----
-            if (ok) ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, lane, s_abort);
+            if (ok) ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, s_abort);
             s_mx[w][row] = l;  // (the last readers of the maxima arrived at p_full before that product)
             soft_any(2, false);
             tc_fence_after();
+            if (ok && s_poison[k % kNotes])
+                add_not_finite<HD, T>(a, it, v, w, tmem + S::O_COL + uint32_t(w * (HD / 2)) + lane_off);
             const float L = s_mx[0][row] + s_mx[1][row];
             const bool whole = it.u0 == 0 && it.u1 == it.units;
             const float inv = L == 0.f ? 0.f : 1.0f / L;
@@ -803,6 +951,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (s_abort) {  // copies and products in flight end well within this time
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000) {
+        }
+        __syncthreads();
+    }
     if (warp == 0) tmem_dealloc(tmem, kTmem);
 }
 
@@ -869,7 +1023,9 @@ TcArgs tc_args(const PagedAttention& p, const PagedScratch& s) {
     a.group = p.Nq / p.Nkv;
     a.tpt = kM / a.group;
     int64_t g = p.ps / 8;
-    a.box_groups = int(g & -g) < 8 ? int(g & -g) : 8;
+    const int64_t most = (p.Hd == 256 ? Shape<256>::KEYS : kN) / 8;  // a box stays inside a slot
+    a.box_groups = int((g & -g) < most ? (g & -g) : most);
+    a.ps_inv = ~uint64_t(0) / uint64_t(p.ps) + 1;  // (exact quotients for keys and sizes below 2^31)
     a.rows_cap = int(paged_attention_scratch_rows(p));
     a.c = p.scale * kLog2e;
     a.groups = p.P * p.Nkv * p.ps / 8;
