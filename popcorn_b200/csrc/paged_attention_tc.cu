@@ -6,10 +6,11 @@
 // heads that share a KV head share its K/V reads. An item's units are the
 // 128-key tiles that some row of it sees: those of the sink tokens, then
 // those from the first row's window start to the last row's position.
-// Every CTA of one wave takes an equal run of consecutive units — ragged
-// lengths, long contexts with one token and long chunks all fill the GPU —
-// and cuts an item where its run ends; the pieces' (m, l, O) go to scratch
-// and a second kernel joins them in order (the cut depends on the lengths
+// Every CTA of one wave takes an equal run of consecutive units (an item also
+// counts for one, its epilogue's share), cutting an item where its run ends
+// unless the item's own end is near: ragged lengths, long contexts with one
+// token and long chunks all fill the GPU. The pieces' (m, l, O) go to scratch
+// and a second kernel joins them in order (the cuts depend on the lengths
 // alone, so results repeat bit for bit). The plan is computed by every CTA
 // from the lengths on the device.
 //
@@ -17,16 +18,17 @@
 // (128-byte swizzle, a box per run of page rows); warp 2 loads V; both fill
 // one ring in the order K(0), K(1), V(0), K(2), V(1), ...; warp 1 issues S = Q.K^T
 // into the next of NS accumulators in tensor memory and O += P.V, whichever
-// is ready; warps 4-11 (two threads a row, 64 keys each) turn S into P =
-// 2^(c S - m): P is packed into the type and written back over S, from where
-// the second product reads it as its A operand, so it never passes through
-// shared memory. A ring slot holds 8-key groups of [Hd/64][8 keys][128 B], so
+// is ready; warps 4-7 and 8-11 take tiles in turn (a thread a row) and turn S
+// into P = 2^(c S - m): P is packed into the type and written back over S,
+// from where the second product reads it as its A operand, so it never passes
+// through shared memory; one group's loads and waits pass under the other's
+// exponentials (the MUFU's 16 a clock are the bound: 1024 clocks a tile). A ring slot holds 8-key groups of [Hd/64][8 keys][128 B], so
 // any page size that is a multiple of 8 gives one layout (group stride Hd/64
 // KB) and the two halves of a tile in neighbouring slots are one operand.
 //
 // The running max is kept until it grows by more than 2^8 (P <= 256 then; O
-// and l use the same max, so O / l is exact for any); the two threads of a
-// row and all rows agree on that by one barrier vote a tile. P is rounded to
+// and l use the same max, so O / l is exact for any); it goes from group to
+// group with the tiles, warp to warp. P is rounded to
 // the type once: as far from the exact weights as the output's own rounding
 // is from the exact output (half a step each); sums, m, l and O are fp32.
 //
@@ -59,7 +61,7 @@ using namespace tc;
 constexpr int kM = 128;          // query rows of an item
 constexpr int kN = 128;          // keys of a unit
 constexpr int kPtThreads = 384;  // warps: 0 Q and K loads, 1 MMA, 2 V loads, 3 masked V, 4-11 softmax
-constexpr int kSoftThreads = 256;
+constexpr int kSoftWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 of the growth of a row's max that is let pass
 constexpr uint32_t kTmem = 512;
@@ -75,11 +77,11 @@ struct Shape {
     static constexpr int NSLOT = HD == 256 ? 5 : (HD == 128 ? 6 : 10);
     // Warp 0's notes on items and units, a ring. It writes note j with K(j - 1)
     // in the ring, so K(j - 1 - T) has been read (T tiles fit the ring), which
-    // waited for the product j - 1 - T - NS: entries up to there are free
-    // (Hd 256, whose odd ring mixes K and V: up to j - 4). Warp 3, idle where
-    // nothing is masked, hands its entries back.
-    static constexpr int NOTES = HD == 64 ? 16 : 8;
-    static_assert(HD == 256 || NOTES >= NSLOT / 2 + NS + 1, "notes outlive their readers");
+    // waited for the product j - 1 - T - NS, and both softmax groups are done
+    // with the tile two before that (Hd 256, whose odd ring mixes K and V:
+    // product j - 4). Warp 3, idle where nothing is masked, hands its entries
+    // back.
+    static constexpr int NOTES = HD == 256 ? 6 : NSLOT / 2 + NS + 3;
     static constexpr int Q_BLOCK = kM * 128;
     static constexpr int Q_BYTES = ATOMS * Q_BLOCK;
     static constexpr uint32_t O_COL = NS * kN;
@@ -104,8 +106,8 @@ struct TcArgs {
     int rows_cap;   // rows of a scratch slot
     float c;        // scale * log2(e)
     int64_t groups; // 8-row groups of the pages (past the end: zero fill)
-    float* po;      // [2 * CTAs][rows_cap][HD]
-    float* pml;     // [2 * CTAs][rows_cap][2]
+    float* po;      // [2 * CTAs][HD / 4][rows_cap][4]
+    float* pml;     // [2 * CTAs][2][rows_cap]: m, l
     Cut* cuts;      // [CTAs]
 };
 
@@ -118,7 +120,7 @@ struct Item {
     int lo, hi, sink;  // keys that some row sees: [0, sink) and [lo, hi)
     int t_lo, ns, units;  // tiles [0, ns) and from t_lo on
     int u0, u1;           // this CTA's share
-    int64_t start;        // the item's first unit in the step's order
+    int64_t start, end;   // where the item lies in the step's order
 };
 
 // (Not inlined: the roles' loops are long, and the instruction cache is what they share.)
@@ -142,54 +144,69 @@ __device__ __noinline__ void item_span(const TcArgs& a, const Request& rq, int m
     it.units = u > 1 ? u : 1;  // (rows without a key are written too)
 }
 
-struct Start {
-    int r, h, mt, u;
-    int64_t unit, left;
+// A place in the step's order: `at`, `off` into item (r, h, mt), which starts
+// at `at - off` and counts `cost`.
+struct Place {
+    int r, h, mt, off;
+    int64_t at, cost;
+};
+struct Plan {
+    Place begin;
+    int64_t end;    // of this CTA's run
+    int64_t total;  // of the step
+    int ctas;       // that have a run
+    int extra;      // what an item counts besides its units
+    int near;       // a cut this near to an end of its item moves there
 };
 
-// The CTA's items in order (walked by the load warp, which tells the others).
+// Where the cut at place x of an item [s, e) goes.
+__device__ __forceinline__ int64_t moved(int64_t x, int64_t s, int64_t e, int near) {
+    return x - s <= near ? s : (e - x <= near ? e : x);
+}
+
+// The CTA's items in order (walked by warp 0, which tells the others).
 struct Walk {
     const TcArgs& a;
     Request rq;
-    int r, h, mt, u, ntiles;
-    int64_t unit, left;
+    int r, h, mt, off, ntiles, extra;
+    int64_t at, end;
 
-    __device__ __forceinline__ Walk(const TcArgs& args, const Start& s)
-        : a(args), r(s.r), h(s.h), mt(s.mt), u(s.u), unit(s.unit), left(s.left) {
-        if (left > 0) load();
+    __device__ __forceinline__ Walk(const TcArgs& args, const Plan& s)
+        : a(args), r(s.begin.r), h(s.begin.h), mt(s.begin.mt), off(s.begin.off), extra(s.extra), at(s.begin.at), end(s.end) {
+        if (at < end) load();
     }
     __device__ __forceinline__ void load() {
         rq = request(a.p, r);
         ntiles = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
     }
     __device__ __noinline__ bool next(Item& it) {
-        if (left <= 0) return false;
-        item_span(a, rq, mt, it);
-        it.r = r;
-        it.h = h;
-        it.u0 = u;
-        it.u1 = it.units - u <= left ? it.units : u + int(left);
-        it.start = unit - u;
-        unit += it.u1 - u;
-        left -= it.u1 - u;
-        if (it.u1 < it.units) {
-            u = it.u1;  // (left is 0)
-            return true;
-        }
-        u = 0;
-        if (++mt == ntiles) {
-            mt = 0;
-            if (++h == a.p.Nkv) {
-                h = 0;
-                if (left > 0) {
-                    do ++r;
-                    while (r < a.p.R && request(a.p, r).n == 0);
-                    if (r < a.p.R) load();
-                    else left = 0;
+        while (at < end) {
+            item_span(a, rq, mt, it);
+            it.r = r;
+            it.h = h;
+            it.start = at - off;
+            it.end = it.start + it.units + extra;
+            const int64_t stop = it.end < end ? it.end : end;
+            it.u0 = off > extra ? off - extra : 0;
+            const int64_t u1 = stop - it.start - extra;
+            it.u1 = u1 > 0 ? int(u1) : 0;
+            at = stop;
+            off = 0;
+            if (++mt == ntiles) {
+                mt = 0;
+                if (++h == a.p.Nkv) {
+                    h = 0;
+                    if (at < end) {
+                        do ++r;
+                        while (r < a.p.R && request(a.p, r).n == 0);
+                        if (r < a.p.R) load();
+                        else at = end;
+                    }
                 }
             }
+            if (it.u1 > it.u0) return true;
         }
-        return true;
+        return false;
     }
 };
 
@@ -213,9 +230,15 @@ __device__ __forceinline__ bool guarded(const TcArgs& a, const Item& it, int64_t
 }
 
 // What warp 0 says of a unit.
-enum : int { kFirst = 1, kLast = 2, kLook = 4 };  // first / last of its item here; kLook << h: half h is guarded
+enum : int {
+    kFirst = 1, kLast = 2,  // of its item in this CTA
+    kOpen = 4,              // every row sees every key of the tile
+    kStop = 8,              // no unit: the CTA is done
+    kLook = 16              // kLook << h: half h of V is guarded
+};
 struct Unit {
     int flags;
+    int tile;       // its keys: from tile * 128 on
     int group[16];  // of each box: its first 8-row group of the pages, past the last one for zeros
 };
 
@@ -227,8 +250,27 @@ __device__ __forceinline__ float ex2(float x) {
 
 // 64 consecutive fp32 columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld64(uint32_t addr, float2* v) {
-    tmem_ld32(addr, reinterpret_cast<float*>(v));
-    tmem_ld32(addr + 32, reinterpret_cast<float*>(v) + 32);
+    uint32_t r[64];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 
 // Two fp32 operations in one instruction.
@@ -291,20 +333,6 @@ __device__ __forceinline__ bool wait_bar(uint64_t& bar, uint32_t parity, volatil
     return wait_long(b, parity, &abort);
 }
 
-// Barrier `id` over the softmax threads; true where any of them says so.
-__device__ __forceinline__ bool soft_any(int id, bool mine) {
-    uint32_t any;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(any)
-        : "r"(uint32_t(mine)), "r"(id), "r"(kSoftThreads)
-        : "memory");
-    return any != 0;
-}
-
 // Exponent fields of two 16-bit values: bit 15 of a half is set in the result where its value is not finite.
 template <class T>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
@@ -362,12 +390,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     constexpr bool BF = T::code == TBF16::code;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t item_full[kNotes], unit_full[kNotes], unit_free[kNotes], look[kNotes], q_full, q_empty,
-        full[NSLOT], empty[NSLOT], s_full[NS], p_full[NS], pv_done[NS], o_free;
+        full[NSLOT], empty[NSLOT], s_full[NS], p_full[NS], pv_done[NS], o_free, m_ready[2][4], l_ready[2][4];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
-    __shared__ Start s_start;
-    __shared__ long long s_scan[kPtThreads / 32];
-    __shared__ float s_mx[2][kM];  // a row's two maxima, at an item's end its two sums
+    __shared__ Plan s_plan;
+    __shared__ float s_m[kM], s_l[kM];  // rows' running maxima (at an item's end their sums), the other group's sums
     __shared__ Item s_item[kNotes];
     __shared__ volatile int s_poison[kNotes];  // an item has V values that are not finite in a tile with masked keys
     __shared__ Unit s_unit[kNotes];
@@ -398,115 +425,173 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (int i = 0; i < NS; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&pv_done[i]), 1);
-            mbar_init(smem_u32(&p_full[i]), kSoftThreads / 32);
+            mbar_init(smem_u32(&p_full[i]), kSoftWarps / 2);
         }
-        mbar_init(smem_u32(&o_free), kSoftThreads / 32);
+        for (int i = 0; i < 8; ++i) {
+            mbar_init(smem_u32(&m_ready[i >> 2][i & 3]), 1);
+            mbar_init(smem_u32(&l_ready[i >> 2][i & 3]), 1);
+        }
+        mbar_init(smem_u32(&o_free), kSoftWarps);
         s_abort = 0;
         mbar_fence_init();
     }
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), kTmem);
     pdl_wait();
 
-    // ---- the plan: sums of the requests' units, and where this CTA begins ----
+    // ---- the plan: sums of the requests' units, and where this CTA's run begins and ends ----
     long long* cum = reinterpret_cast<long long*>(ring);  // [R + 1], before any copy uses the ring
+    long long* scan = reinterpret_cast<long long*>(sq);   // [2 * warps]
+    auto tiles_of = [&](const Request& rq) { return int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt)); };
     auto head_units = [&](const Request& rq, int from, int step) {
         long long u = 0;
-        const int nt = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
+        const int nt = tiles_of(rq);
         Item it;
+#pragma unroll 1
         for (int mt = from; mt < nt; mt += step) {
             item_span(a, rq, mt, it);
             u += it.units;
         }
         return u;
     };
-    if (p.R <= 8 * (kPtThreads / 32)) {  // a warp a request: long chunks have many tiles
-        for (int r = warp; r < p.R; r += kPtThreads / 32) {
-            long long u = head_units(request(p, r), lane, 32);
+    const bool by_warp = p.R <= 8 * (kPtThreads / 32);  // a warp a request: long chunks have many tiles
+#pragma unroll 1
+    for (int r = by_warp ? warp : tid; r < p.R; r += by_warp ? kPtThreads / 32 : kPtThreads) {
+        long long u = head_units(request(p, r), by_warp ? lane : 0, by_warp ? 32 : 1);
+        if (by_warp) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-            if (lane == 0) cum[r + 1] = u * p.Nkv;
         }
-    } else {
-        for (int r = tid; r < p.R; r += kPtThreads) cum[r + 1] = head_units(request(p, r), 0, 1) * p.Nkv;
+        if (!by_warp || lane == 0) cum[r + 1] = u * p.Nkv;
     }
     if (tid == 0) cum[0] = 0;
     __syncthreads();
     {
+        // each thread sums a run of requests, units and items
         const int per = (p.R + kPtThreads - 1) / kPtThreads;
         const int r0 = tid * per < p.R ? tid * per : p.R, r1 = r0 + per < p.R ? r0 + per : p.R;
-        long long sum = 0;
-        for (int r = r0; r < r1; ++r) sum += cum[r + 1];
-        long long incl = sum;
+        long long sum = 0, items = 0;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            sum += cum[r + 1];
+            items += (long long)tiles_of(request(p, r)) * p.Nkv;
+        }
+        long long iu = sum, ii = items;  // inclusive over the warp
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
+            const long long x = __shfl_up_sync(0xffffffffu, iu, o), y = __shfl_up_sync(0xffffffffu, ii, o);
+            if (lane >= o) {
+                iu += x;
+                ii += y;
+            }
         }
-        if (lane == 31) s_scan[warp] = incl;
+        if (lane == 31) {
+            scan[warp] = iu;
+            scan[kPtThreads / 32 + warp] = ii;
+        }
         __syncthreads();
-        long long run = incl - sum;
-        for (int w = 0; w < warp; ++w) run += s_scan[w];
+        long long run = iu - sum, run_items = ii - items, units = 0;
+        for (int x = 0; x < kPtThreads / 32; ++x) {
+            if (x < warp) {
+                run += scan[x];
+                run_items += scan[kPtThreads / 32 + x];
+            }
+            units += scan[x];
+        }
+        // With runs long enough, an item counts for its epilogue too, and cuts keep clear of its ends.
+        const int extra = units >= 16ll * gridDim.x ? 1 : 0;
+        run += extra * run_items;
+#pragma unroll 1
         for (int r = r0; r < r1; ++r) {
-            run += cum[r + 1];
+            run += cum[r + 1] + (extra ? (long long)tiles_of(request(p, r)) * p.Nkv : 0);
             cum[r + 1] = run;
+        }
+        if (tid == 0) {
+            s_plan.extra = extra;
+            s_plan.near = extra ? 3 : 0;
         }
     }
     __syncthreads();
-    const long long U = cum[p.R];
-    const long long ctas = U < (long long)gridDim.x ? U : (long long)gridDim.x;
-    if (warp == 0) {
-        Start s{0, 0, 0, 0, 0, 0};
-        if ((long long)blockIdx.x < ctas) {
-            const long long u = blockIdx.x * U / ctas;
-            s.unit = u;
-            s.left = (blockIdx.x + 1) * U / ctas - u;
+    if (warp < 2) {
+        // warp 0: where the run begins, warp 1: where it ends
+        const long long U = cum[p.R];
+        const int ctas = U < (long long)gridDim.x ? int(U) : int(gridDim.x);
+        Place b{0, 0, 0, 0, U, 0};
+        const int c = int(blockIdx.x) + warp;
+        if (c < ctas) {
+            const long long x = c * U / ctas;
             int lo = 0, hi = p.R;
+#pragma unroll 1
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (cum[mid] <= u) lo = mid;
+                if (cum[mid] <= x) lo = mid;
                 else hi = mid;
             }
-            s.r = lo;
             const long long per_head = (cum[lo + 1] - cum[lo]) / p.Nkv;
-            long long rem = u - cum[lo];
-            s.h = int(rem / per_head);
-            rem -= s.h * per_head;
+            long long rem = x - cum[lo];
+            b.r = lo;
+            b.h = int(rem / per_head);
+            rem -= b.h * per_head;
             // the item: 32 tiles at a time
             const Request rq = request(p, lo);
-            const int nt = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
+            const int nt = tiles_of(rq);
+#pragma unroll 1
             for (int mt0 = 0; mt0 < nt; mt0 += 32) {
                 Item it;
                 it.units = 0;
-                if (mt0 + lane < nt) item_span(a, rq, mt0 + lane, it);
+                if (mt0 + lane < nt) {
+                    item_span(a, rq, mt0 + lane, it);
+                    it.units += s_plan.extra;
+                }
                 long long incl = it.units;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += x;
+                    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += y;
                 }
                 const unsigned hit = __ballot_sync(0xffffffffu, incl > rem);
                 if (hit) {
                     const int l = __ffs(int(hit)) - 1;
-                    s.mt = mt0 + l;
-                    s.u = int(rem - __shfl_sync(0xffffffffu, incl - it.units, l));
+                    b.mt = mt0 + l;
+                    b.off = int(rem - __shfl_sync(0xffffffffu, incl - it.units, l));
+                    b.cost = __shfl_sync(0xffffffffu, it.units, l);
                     break;
                 }
                 rem -= __shfl_sync(0xffffffffu, incl, 31);
             }
+            const long long s0 = x - b.off, to = moved(x, s0, s0 + b.cost, s_plan.near);
+            b.at = to;
+            b.off = int(to - s0);
+            if (to == s0 + b.cost) {  // the next item
+                b.off = 0;
+                if (++b.mt == nt) {
+                    b.mt = 0;
+                    if (++b.h == p.Nkv) {
+                        b.h = 0;
+#pragma unroll 1
+                        do ++b.r;
+                        while (b.r < p.R && request(p, b.r).n == 0);
+                    }
+                }
+            }
         }
-        if (lane == 0) s_start = s;
+        if (lane == 0) {
+            if (warp == 0) {
+                s_plan.begin = b;
+                s_plan.total = U;
+                s_plan.ctas = ctas;
+            } else {
+                s_plan.end = b.at;
+            }
+        }
     }
     tc_fence_before();
     fence_async_smem();  // the sums' readers are done before copies land there
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const Start start = s_start;
-
-    const int n = int(start.left);  // units of this CTA
     constexpr int H = S::HALVES;    // ring positions of a K or V tile, from k_pos / v_pos on
     auto k_pos = [&](int j) { return j == 0 ? 0 : (2 * j - 1) * H; };
-    auto v_pos = [&](int j) { return (j == n - 1 ? 2 * n - 1 : 2 * j + 2) * H; };
+    auto v_pos = [&](int j) { return (2 * j + 2) * H; };
     // Item k of this CTA, once warp 0 has published it.
     auto item = [&](int k, Item& it) {
         if (!wait_bar(item_full[k % kNotes], uint32_t(k / kNotes) & 1u, s_abort)) return false;
@@ -537,7 +622,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
     if (warp == 0) {
         // ---- items, pages, Q and K ----
-        Walk walk(a, start);
+        Walk walk(a, s_plan);
         bool ok = true;
         const int box_keys = a.box_groups * 8;
         const int per_fill = 32 / boxes;  // units whose boxes one look at the table covers
@@ -563,7 +648,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         };
         Item it, nx;  // the item at hand, and the one of the next look
         int items = 0, nu = 0, page = -1, j = 0;
-        bool more = n > 0 && walk.next(nx);
+        bool more = walk.next(nx);
         if (more) {
             nu = nx.u0;
             page = page_of(nx, nu);
@@ -587,10 +672,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 if (my_unit == u - u_first) note.group[my_box] = g;
                 __syncwarp();
                 if (lane == 0) {
-                    int flags = (u == it.u0 ? kFirst : 0) | (u == it.u1 - 1 ? kLast : 0);
+                    const int64_t key0 = int64_t(tile_of(it, u)) * kN;
+                    int flags = (u == it.u0 ? kFirst : 0) | (u == it.u1 - 1 ? kLast : 0) |
+                                (keys_open(a, it, key0, kN) ? kOpen : 0);
+                    note.tile = tile_of(it, u);
 #pragma unroll
                     for (int h = 0; h < H; ++h)
-                        if (guarded(a, it, int64_t(tile_of(it, u)) * kN + h * S::KEYS, S::KEYS)) flags |= kLook << h;
+                        if (!(flags & kOpen) && guarded(a, it, key0 + h * S::KEYS, S::KEYS)) flags |= kLook << h;
                     note.flags = flags;
                     if (u == it.u0) {
                         s_poison[items % kNotes] = 0;
@@ -617,15 +705,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 ok = put(note.group, k_pos(j), none, &map_k);
             }
         }
+        if (ok) ok = wait_bar(unit_free[j % kNotes], (uint32_t(j / kNotes) & 1u) ^ 1u, s_abort);
+        if (ok && lane == 0) {
+            s_unit[j % kNotes].flags = kStop;
+            mbar_arrive(smem_u32(&unit_full[j % kNotes]));
+        }
         if (!ok) s_abort = 1;
     } else if (warp == 2) {
         // ---- V ----
         bool ok = true;
         int looks = 0;
-        for (int j = 0; j < n && ok; ++j) {
+        for (int j = 0; ok; ++j) {
             ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
-            if (!ok) break;
             const Unit& note = s_unit[j % kNotes];
+            if (!ok || (note.flags & kStop)) break;
             uint64_t* to[2] = {nullptr, nullptr};
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -634,7 +727,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (!ok) s_abort = 1;
     } else if (warp == 1) {
-        if (lane == 0 && n > 0) {
+        if (lane == 0) {
             // ---- MMA issue ----
             constexpr uint32_t idesc_s = make_idesc(BF, kM, kN, false), idesc_h = make_idesc(BF, kM, kN / 2, false);
             constexpr uint32_t idesc_o = make_idesc(BF, kM, HD, true);
@@ -645,16 +738,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             int ns = 0, np = 0;  // next tile of S, of O
             int ks = 0, kp = 0;  // their items
             int fs = 0;          // the notes on tile ns (0: not read yet)
-            bool ok = true;
+            bool ok = true, stop = false;
             uint32_t idle = 0;
-            while (np < n && !s_abort) {
+            while (!(stop && np == ns) && !s_abort) {
                 bool progressed = false;
-                if (ns < n && ns < np + NS) {
+                if (!stop && ns < np + NS) {
                     const int buf = ns % NS;
                     const int q0 = k_pos(ns), q1 = q0 + H - 1;
                     if (fs == 0 && mbar_test_wait(smem_u32(&unit_full[ns % kNotes]), uint32_t(ns / kNotes) & 1u))
                         fs = s_unit[ns % kNotes].flags | 256;
-                    if (fs && (ns < NS || mbar_test_wait(smem_u32(&pv_done[buf]), uint32_t(ns / NS - 1) & 1u)) &&
+                    stop = fs & kStop;
+                    if (fs && !stop && (ns < NS || mbar_test_wait(smem_u32(&pv_done[buf]), uint32_t(ns / NS - 1) & 1u)) &&
                         (!(fs & kFirst) || mbar_test_wait(smem_u32(&q_full), uint32_t(ks) & 1u)) && is_full(q0) &&
                         (H == 1 || is_full(q1))) {
                         tc_fence_after();
@@ -702,7 +796,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                             const uint64_t db = desc_mn(v, S::GROUP);
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)
-                                tc_mma_ts(tmem + S::O_COL, pa + (4 * h + kk) * 8, db + uint64_t(kk * (2 * S::GROUP >> 4)), idesc_o,
+                                tc_mma_ts(tmem + S::O_COL, pa + h * 64 + kk * 8, db + uint64_t(kk * (2 * S::GROUP >> 4)), idesc_o,
                                           (!first || h > 0 || kk > 0) ? 1u : 0u);
                         }
                         tc_commit(smem_u32(&empty[s0]));
@@ -728,22 +822,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         Item it;
         bool ok = true;
         int looks = 0;
-        for (int j = 0, k = -1; j < n && ok; ++j) {
+        for (int j = 0, k = -1; ok; ++j) {
             ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
-            if (!ok) break;
-            const int flags = s_unit[j % kNotes].flags;
+            const int flags = s_unit[j % kNotes].flags, tile = s_unit[j % kNotes].tile;
+            if (!ok || (flags & kStop)) break;
             if (flags & kFirst) {
                 ok = item(++k, it);
                 if (!ok) break;
-                it.units = it.u0;  // (here: the unit at hand)
-            } else {
-                ++it.units;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&unit_free[j % kNotes]));
             for (int h = 0; h < H && ok; ++h) {
                 if (!(flags & (kLook << h))) continue;
-                const int64_t key0 = int64_t(tile_of(it, it.units)) * kN + h * S::KEYS;
+                const int64_t key0 = int64_t(tile) * kN + h * S::KEYS;
                 const int slot = (v_pos(j) + h) % NSLOT;
                 ok = wait_bar(look[looks % kNotes], uint32_t(looks / kNotes) & 1u, s_abort);
                 ++looks;
@@ -785,168 +876,230 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (!ok) s_abort = 1;
     } else if (warp >= 4) {
-        // ---- softmax: row (warp % 4) * 32 + lane, keys [64 w, 64 w + 64) of each tile ----
+        // ---- softmax: a thread a row; group w takes the tiles with j % 2 == w ----
         const int w = (warp - 4) >> 2;
-        const int quarter = warp & 3;
+        const int quarter = warp & 3;  // TMEM lanes this warp may access
         const int row = quarter * 32 + lane;
-        const int soft = (warp - 4) * 32 + lane;
         const uint32_t lane_off = uint32_t(quarter * 32) << 16;
         const int ti = row / a.group, gi = row % a.group;
         Item it;
-        bool ok = true;  // (once false, the barriers below are still met, so that no warp is left at one)
-        int j = 0;
+        Span v{0, 0, 0};
+        bool ok = true, valid = false, live = false;
+        int k = -1;
+        float m = -INFINITY, l = 0.f;  // l: this group's share, under m
         Cut cut{0, 0, 0, -1, 0};
-        for (int k = 0; j < n; ++k) {
-            if (ok) ok = item(k, it);
-            if (soft_any(2, !ok)) {  // (all leave together)
-                ok = false;
-                break;
+        for (int j = 0; ok; ++j) {
+            ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
+            const int flags = s_unit[j % kNotes].flags;
+            if (!ok || (flags & kStop)) break;
+            if (flags & kFirst) {
+                ok = item(++k, it);
+                if (!ok) break;
+                const int rows = it.ntok * a.group;
+                valid = row < rows;
+                live = quarter * 32 < rows;  // some row of the warp is there
+                v = visible(p, Request{it.tok0, it.ntok, it.len}, int64_t(it.pos0) + ti);
+                if (!valid) v = Span{0, 0, 0};
+                m = -INFINITY;
+                l = 0.f;
             }
-            const int rows = it.ntok * a.group;
-            const bool valid = row < rows;
-            const bool live = quarter * 32 < rows;  // some row of the warp is there
-            Span v = visible(p, Request{it.tok0, it.ntok, it.len}, int64_t(it.pos0) + ti);
-            if (!valid) v = Span{0, 0, 0};
-            float m = -INFINITY, l = 0.f;
-            for (int u = it.u0; u < it.u1; ++u, ++j) {
-                const int buf = j % NS;
-                const int64_t key0 = int64_t(tile_of(it, u)) * kN + w * 64;  // this thread's 64 keys
-                const bool open = keys_open(a, it, key0, 64);
-                if (ok) ok = wait_bar(s_full[buf], uint32_t(j / NS) & 1u, s_abort);
+            const int buf = j % NS;
+            if ((j & 1) == w) {
+                ok = wait_bar(s_full[buf], uint32_t(j / NS) & 1u, s_abort);
+                if (!ok) break;
                 tc_fence_after();
                 float2 s[32];
                 float mx = -INFINITY;
-                if (ok && live) {
-                    tmem_ld64(tmem + uint32_t(buf * kN + w * 64) + lane_off, s);
-                    if (!open) {
-                        // bit c: this row sees key c of the thread's 64
-                        auto below = [&](int64_t x) {
-                            const int64_t n = x - key0;
-                            return n <= 0 ? uint64_t(0) : (n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1);
-                        };
-                        const uint64_t sees = (below(v.hi) & ~below(v.lo)) | below(v.sink);
-                        const uint32_t bits[2] = {uint32_t(sees), uint32_t(sees >> 32)};
+                const int64_t key0 = int64_t(s_unit[j % kNotes].tile) * kN;
+                // Keys [64 h, 64 h + 64) of the tile; both passes read them from tensor memory.
+                auto load = [&](int h) {
+                    tmem_ld64(tmem + uint32_t(buf * kN + h * 64) + lane_off, s);
+                    if (flags & kOpen) return;
+                    // bit c: this row sees key c of them
+                    auto below = [&](int64_t x) {
+                        const int64_t n = x - (key0 + h * 64);
+                        return n <= 0 ? uint64_t(0) : (n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1);
+                    };
+                    const uint64_t sees = (below(v.hi) & ~below(v.lo)) | below(v.sink);
+                    const uint32_t bits[2] = {uint32_t(sees), uint32_t(sees >> 32)};
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            if (!(bits[c >> 4] & (1u << (2 * (c & 15))))) s[c].x = -INFINITY;
-                            if (!(bits[c >> 4] & (2u << (2 * (c & 15))))) s[c].y = -INFINITY;
-                        }
+                    for (int c = 0; c < 32; ++c) {
+                        if (!(bits[c >> 4] & (1u << (2 * (c & 15))))) s[c].x = -INFINITY;
+                        if (!(bits[c >> 4] & (2u << (2 * (c & 15))))) s[c].y = -INFINITY;
                     }
-                    float m0 = s[0].x, m1 = s[0].y, m2 = s[1].x, m3 = s[1].y;
-#pragma unroll
-                    for (int c = 2; c < 32; c += 2) {
-                        m0 = fmaxf(m0, s[c].x);
-                        m1 = fmaxf(m1, s[c].y);
-                        m2 = fmaxf(m2, s[c + 1].x);
-                        m3 = fmaxf(m3, s[c + 1].y);
-                    }
-                    mx = fmaxf(mx, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.c);
-                }
-                if (soft_any(1, ok && valid && mx > m + kGrow)) {
-                    s_mx[w][row] = mx;
-                    soft_any(2, false);
-                    const float both = fmaxf(s_mx[0][row], s_mx[1][row]);
-                    float f = 1.f;
-                    if (valid && both > m + kGrow) {
-                        f = m == -INFINITY ? 0.f : ex2(m - both);
-                        m = both;
-                        l *= f;
-                    }
-                    if (ok && u > it.u0 && __any_sync(0xffffffffu, f != 1.f)) {
-                        // O was accumulated under the old max
-                        ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, s_abort);
-                        tc_fence_after();
-                        if (ok) {
-                            // (f 0: a row whose keys so far weighed nothing; its O is zero)
-                            const float g = f == 0.f ? 1.f : f;
+                };
+                if (live) {
 #pragma unroll 1
-                            for (int cc = 0; cc < HD / 64; ++cc) {
-                                float o[32];
-                                const uint32_t at = tmem + S::O_COL + uint32_t(w * (HD / 2) + cc * 32) + lane_off;
-                                tmem_ld32(at, o);
+                    for (int h = 0; h < 2; ++h) {
+                        load(h);
+                        float m0 = s[0].x, m1 = s[0].y, m2 = s[1].x, m3 = s[1].y;
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] *= g;
-                                tmem_st32(at, o);
-                            }
-                            tmem_wait_st();
+                        for (int c = 2; c < 32; c += 2) {
+                            m0 = fmaxf(m0, s[c].x);
+                            m1 = fmaxf(m1, s[c].y);
+                            m2 = fmaxf(m2, s[c + 1].x);
+                            m3 = fmaxf(m3, s[c + 1].y);
                         }
+                        mx = fmaxf(mx, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.c);
                     }
                 }
-                if (ok && live) {
+                // the running max, from the tile before (another item's is of no use, but its turn is awaited)
+                if (j > 0) {
+                    ok = wait_bar(m_ready[w ^ 1][quarter], uint32_t((j - 1) >> 1) & 1u, s_abort);
+                    if (!ok) break;
+                }
+                const bool first = flags & kFirst;
+                const float before = first ? -INFINITY : s_m[row];
+                float now = before;
+                if (valid && mx > before + kGrow) now = mx;
+                s_m[row] = now;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&m_ready[w][quarter]));
+                if (now != m) {
+                    if (m != -INFINITY) l *= ex2(m - now);
+                    m = now;
+                }
+                if (live) {
                     const float mu = m == -INFINITY ? 0.f : m;
                     const float2 c2 = make_float2(a.c, a.c), m2 = make_float2(-mu, -mu);
                     float2 sum0 = make_float2(l, 0.f), sum1 = make_float2(0.f, 0.f);
-                    float pk[32];
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        load(h);
+                        float pk[32];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        float2 x = fma2(s[c], c2, m2);
-                        x.x = ex2(x.x);
-                        x.y = ex2(x.y);
-                        if (c & 1) sum1 = add2(sum1, x);
-                        else sum0 = add2(sum0, x);
-                        pk[c] = __uint_as_float(cvt_pair<T>(x.x, x.y));
+                        for (int c = 0; c < 32; ++c) {
+                            float2 x = fma2(s[c], c2, m2);
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
+                            if (c & 1) sum1 = add2(sum1, x);
+                            else sum0 = add2(sum0, x);
+                            pk[c] = __uint_as_float(cvt_pair<T>(x.x, x.y));
+                        }
+                        // over the scores that it came from
+                        tmem_st32(tmem + uint32_t(buf * kN + h * 64) + lane_off, pk);
                     }
                     sum0 = add2(sum0, sum1);
                     l = sum0.x + sum0.y;
-                    tmem_st32(tmem + uint32_t(buf * kN + w * 32) + lane_off, pk);
+                    tmem_wait_st();
+                }
+                if (!first && __any_sync(0xffffffffu, now != before && before != -INFINITY)) {
+                    // O was accumulated under the old max
+                    ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, s_abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float f = now != before && before != -INFINITY ? ex2(before - now) : 1.f;
+#pragma unroll 1
+                    for (int cc = 0; cc < HD / 32; ++cc) {
+                        float o[32];
+                        const uint32_t at = tmem + S::O_COL + uint32_t(cc * 32) + lane_off;
+                        tmem_ld32(at, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= f;
+                        tmem_st32(at, o);
+                    }
                     tmem_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&p_full[buf]));
             }
-            // ---- the item's share is summed: O / l, or its piece ----
-            if (ok) ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, s_abort);
-            s_mx[w][row] = l;  // (the last readers of the maxima arrived at p_full before that product)
-            soft_any(2, false);
+            if (!(flags & kLast)) continue;
+            // ---- the item's share is summed: O / l, or its piece; group w has half of the columns ----
+            ok = wait_bar(pv_done[buf], uint32_t(j / NS) & 1u, s_abort);
+            if (ok && (j & 1) != w) ok = wait_bar(m_ready[w ^ 1][quarter], uint32_t(j >> 1) & 1u, s_abort);
+            if (!ok) break;
             tc_fence_after();
-            if (ok && s_poison[k % kNotes])
-                add_not_finite<HD, T>(a, it, v, w, tmem + S::O_COL + uint32_t(w * (HD / 2)) + lane_off);
-            const float L = s_mx[0][row] + s_mx[1][row];
+            const float last_m = s_m[row];
+            if (m != last_m && m != -INFINITY) l *= ex2(m - last_m);
+            // the group without the last tile gives its share, the other one the sum of both
+            float L;
+            if ((j & 1) != w) {
+                s_l[row] = l;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&l_ready[0][quarter]));
+                ok = wait_bar(l_ready[1][quarter], uint32_t(k) & 1u, s_abort);
+                L = s_m[row];
+            } else {
+                ok = wait_bar(l_ready[0][quarter], uint32_t(k) & 1u, s_abort);
+                L = l + s_l[row];
+                s_m[row] = L;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&l_ready[1][quarter]));
+            }
+            if (!ok) break;
+            const uint32_t o_addr = tmem + S::O_COL + uint32_t(w * (HD / 2)) + lane_off;
+            if (s_poison[k % kNotes]) add_not_finite<HD, T>(a, it, v, w, o_addr);
             const bool whole = it.u0 == 0 && it.u1 == it.units;
-            const float inv = L == 0.f ? 0.f : 1.0f / L;
-            const int64_t slot = 2 * int64_t(blockIdx.x) + (it.u0 > 0 ? 0 : 1);
-            uint16_t* dst = static_cast<uint16_t*>(p.out) +
-                            ((it.tok0 + ti) * p.Nq + it.h * a.group + gi) * int64_t(HD) + w * (HD / 2);
-            float* part = a.po + (slot * a.rows_cap + row) * int64_t(HD) + w * (HD / 2);
-            if (ok && live) {
+            if (live && whole) {
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                // 16-byte chunks change places among four neighbouring rows, so that four lanes store 64 bytes of a row
+                const int q = lane & 3;
+                uint16_t* dst = static_cast<uint16_t*>(p.out) +
+                                ((int64_t(it.tok0) + ti) * p.Nq + it.h * a.group + gi) * HD + w * (HD / 2);
 #pragma unroll 1
                 for (int cc = 0; cc < HD / 64; ++cc) {
                     float o[32];
-                    tmem_ld32(tmem + S::O_COL + uint32_t(w * (HD / 2) + cc * 32) + lane_off, o);
-                    if (valid && whole) {
-                        uint4* d4 = reinterpret_cast<uint4*>(dst + cc * 32);
-                        if (L == 0.f) {
+                    tmem_ld32(o_addr + cc * 32, o);
+                    uint32_t x[4][4];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                    for (int e = 0; e < 16; ++e)
+                        x[e >> 2][e & 3] = L == 0.f ? 0u : cvt_pair<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+#pragma unroll
+                    for (int step = 1; step <= 2; step <<= 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (i & step) continue;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t give = q & step ? x[i][e] : x[i | step][e];
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, give, step);
+                                if (q & step) x[i][e] = got;
+                                else x[i | step][e] = got;
+                            }
                         }
+                    }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            d4[e] = make_uint4(cvt_pair<T>(o[8 * e] * inv, o[8 * e + 1] * inv),
-                                               cvt_pair<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                               cvt_pair<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
-                                               cvt_pair<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-                    } else if (valid) {
-                        float4* d4 = reinterpret_cast<float4*>(part + cc * 32);
+                    for (int i = 0; i < 4; ++i) {
+                        uint16_t* to = reinterpret_cast<uint16_t*>(
+                            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & ~3) | i));
+                        if (((row & ~3) | i) < it.ntok * a.group)
+                            *reinterpret_cast<uint4*>(to + cc * 32 + q * 8) = make_uint4(x[i][0], x[i][1], x[i][2], x[i][3]);
+                    }
+                }
+            } else if (live) {
+                const int64_t slot = 2 * int64_t(blockIdx.x) + (it.u0 > 0 ? 0 : 1);
+                // [column / 4][row]: neighbouring rows are neighbours
+                float4* part = reinterpret_cast<float4*>(a.po) + (slot * (HD / 4) + w * (HD / 8)) * a.rows_cap + row;
+#pragma unroll 1
+                for (int cc = 0; cc < HD / 64; ++cc) {
+                    float o[32];
+                    tmem_ld32(o_addr + cc * 32, o);
+                    if (valid) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            d4[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            part[(cc * 8 + e) * a.rows_cap] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
                     __syncwarp();
                 }
-                if (!whole && valid && w == 0) {
-                    a.pml[(slot * a.rows_cap + row) * 2] = m;
-                    a.pml[(slot * a.rows_cap + row) * 2 + 1] = L;
+                if (valid && w == 0) {
+                    a.pml[slot * 2 * a.rows_cap + row] = last_m;
+                    a.pml[(slot * 2 + 1) * a.rows_cap + row] = L;
                 }
             }
-            if (it.u0 == 0 && !whole && ok)
-                cut = Cut{it.tok0, it.ntok, it.h, int32_t(((it.start + it.units) * ctas - 1) / U), 1};
+            if (it.u0 == 0 && !whole && warp == 4) {
+                const Plan& pl = s_plan;
+                int64_t c = (it.end * pl.ctas - 1) / pl.total;
+                const int64_t x = c * pl.total / pl.ctas;
+                if (x > it.start && moved(x, it.start, it.end, pl.near) == it.end) --c;
+                cut = Cut{it.tok0, it.ntok, it.h, int32_t(c), 1};
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&o_free));
         }
         if (!ok) s_abort = 1;
-        if (soft == 0) a.cuts[blockIdx.x] = cut;
+        if (warp == 4 && lane == 0) a.cuts[blockIdx.x] = cut;
     }
     __syncwarp();
     tc_fence_before();
@@ -961,49 +1114,47 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 }
 
 // Joins the pieces of the item that begins in CTA blockIdx.x and was cut
-// there: a warp a row, pieces in CTA order.
+// there, in CTA order: 32 rows (a lane each) by 32 columns (four a warp).
 template <int HD, class T>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(const TcArgs a) {
+    __shared__ uint2 tile[32][9];
     pdl_launch_dependents();
     pdl_wait();
     const Cut cut = a.cuts[blockIdx.x];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.y * 8 + warp;
-    if (!cut.begins || row >= cut.ntok * a.group) return;
-    constexpr int E = HD / 32;
+    const int rows = cut.ntok * a.group, row0 = blockIdx.y * 32, row = row0 + lane;
+    if (!cut.begins || row0 >= rows) return;
     const int first = blockIdx.x, last = cut.last;
-    auto slot = [&](int c) { return (2 * int64_t(c) + (c == first ? 1 : 0)) * a.rows_cap + row; };
-    float M = -INFINITY;
-    for (int c = first + lane; c <= last; c += 32) M = fmaxf(M, a.pml[slot(c) * 2]);
-    M = warp_max(M);
-    float L = 0.f;
-    for (int c = first + lane; c <= last; c += 32) {
-        const float m = a.pml[slot(c) * 2];
-        L += (m == -INFINITY ? 0.f : ex2(m - M)) * a.pml[slot(c) * 2 + 1];
-    }
-    L = warp_sum(L);
-    float o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int c = first; c <= last; ++c) {
-        const float m = a.pml[slot(c) * 2];
-        const float f = m == -INFINITY ? 0.f : ex2(m - M);
-        const float2* src = reinterpret_cast<const float2*>(a.po + slot(c) * HD) + lane;
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-            const float2 x = src[e * 32];
-            o[2 * e] = fmaf(f, x.x, o[2 * e]);
-            o[2 * e + 1] = fmaf(f, x.y, o[2 * e + 1]);
+    auto slot = [&](int c) { return 2 * int64_t(c) + (c == first ? 1 : 0); };
+    if (row < rows) {
+        auto m_of = [&](int c) { return a.pml[slot(c) * 2 * a.rows_cap + row]; };
+        float M = -INFINITY;
+#pragma unroll 8
+        for (int c = first; c <= last; ++c) M = fmaxf(M, m_of(c));
+        float L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int col4 = blockIdx.z * 8 + warp;
+#pragma unroll 8
+        for (int c = first; c <= last; ++c) {
+            const float m = m_of(c), l = a.pml[(slot(c) * 2 + 1) * a.rows_cap + row];
+            const float4 x = reinterpret_cast<const float4*>(a.po)[(slot(c) * (HD / 4) + col4) * a.rows_cap + row];
+            const float f = m == -INFINITY ? 0.f : ex2(m - M);
+            L = fmaf(f, l, L);
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
         }
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
+        tile[lane][warp] = L == 0.f ? make_uint2(0u, 0u)
+                                    : make_uint2(cvt_pair<T>(o.x * inv, o.y * inv), cvt_pair<T>(o.z * inv, o.w * inv));
     }
-    const int ti = row / a.group, gi = row % a.group;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) +
-                                                ((cut.tok0 + ti) * a.p.Nq + cut.head * a.group + gi) * int64_t(HD)) + lane;
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e)
-        dst[e * 32] = L == 0.f ? 0u : cvt_pair<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+    __syncthreads();
+    const int r = row0 + int(threadIdx.x >> 3), q = threadIdx.x & 7;
+    if (r >= rows) return;
+    uint16_t* dst = static_cast<uint16_t*>(a.p.out) +
+                    ((cut.tok0 + r / a.group) * a.p.Nq + cut.head * a.group + r % a.group) * int64_t(HD) + blockIdx.z * 32;
+    reinterpret_cast<uint2*>(dst)[q] = tile[r - row0][q];
 }
 
 bool encode_map(CUtensorMap* map, const void* base, int dtype, const cuuint64_t* dims, const cuuint64_t* strides,
@@ -1065,7 +1216,7 @@ cudaError_t run_tc(const PagedAttention& p, const PagedScratch& sc, cudaStream_t
 template <int HD, class T>
 cudaError_t run_join(const PagedAttention& p, const PagedScratch& sc, cudaStream_t s) {
     const TcArgs a = tc_args(p, sc);
-    return launch_k(paged_attention_join_kernel<HD, T>, dim3(unsigned(sc.ctas), unsigned((a.rows_cap + 7) / 8)), dim3(256), 0,
+    return launch_k(paged_attention_join_kernel<HD, T>, dim3(unsigned(sc.ctas), unsigned((a.rows_cap + 31) / 32), HD / 32), dim3(256), 0,
                     s, a);
 }
 
