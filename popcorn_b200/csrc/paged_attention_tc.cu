@@ -156,11 +156,12 @@ struct Plan {
     int64_t total;  // of the step
     int ctas;       // that have a run
     int extra;      // what an item counts besides its units
-    int near;       // a cut this near to an end of its item moves there
 };
 
-// Where the cut at place x of an item [s, e) goes.
-__device__ __forceinline__ int64_t moved(int64_t x, int64_t s, int64_t e, int near) {
+// Where the cut at place x of an item [s, e) of `rows` rows goes: one near an end moves there. A piece costs the write
+// and the read of (m, l, O) of its rows, in units about a third of one for 32 rows; runs as uneven as that cost more.
+__device__ __forceinline__ int64_t moved(int64_t x, int64_t s, int64_t e, int rows, int extra) {
+    const int near = extra ? rows / 40 : 0;
     return x - s <= near ? s : (e - x <= near ? e : x);
 }
 
@@ -409,6 +410,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedAttention& p = a.p;
 
+    if (tid < 4)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(tid == 0 ? &map_q : (tid == 1 ? &map_q1 : (tid == 2 ? &map_k : &map_v)))
+                     : "memory");
     if (tid == 0) {
         mbar_init(smem_u32(&q_full), 1);
         mbar_init(smem_u32(&q_empty), 1);
@@ -453,15 +457,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         return u;
     };
-    const bool by_warp = p.R <= 8 * (kPtThreads / 32);  // a warp a request: long chunks have many tiles
+    // a thread a request; one of many tiles is left to a warp
+    constexpr int kFewTiles = 4;
+    int many = 0;
 #pragma unroll 1
-    for (int r = by_warp ? warp : tid; r < p.R; r += by_warp ? kPtThreads / 32 : kPtThreads) {
-        long long u = head_units(request(p, r), by_warp ? lane : 0, by_warp ? 32 : 1);
-        if (by_warp) {
+    for (int r = tid; r < p.R; r += kPtThreads) {
+        const Request rq = request(p, r);
+        const bool few = tiles_of(rq) <= kFewTiles;
+        cum[r + 1] = few ? head_units(rq, 0, 1) * p.Nkv : -1;
+        many |= !few;
+    }
+    if (__syncthreads_or(many)) {
+#pragma unroll 1
+        for (int r = warp; r < p.R; r += kPtThreads / 32) {
+            if (cum[r + 1] >= 0) continue;
+            long long u = head_units(request(p, r), lane, 32);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+            __syncwarp();
+            if (lane == 0) cum[r + 1] = u * p.Nkv;
         }
-        if (!by_warp || lane == 0) cum[r + 1] = u * p.Nkv;
     }
     if (tid == 0) cum[0] = 0;
     __syncthreads();
@@ -507,7 +522,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (tid == 0) {
             s_plan.extra = extra;
-            s_plan.near = extra ? 3 : 0;
         }
     }
     __syncthreads();
@@ -558,7 +572,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 }
                 rem -= __shfl_sync(0xffffffffu, incl, 31);
             }
-            const long long s0 = x - b.off, to = moved(x, s0, s0 + b.cost, s_plan.near);
+            const int ntok = rq.n - int64_t(b.mt) * a.tpt < a.tpt ? int(rq.n - int64_t(b.mt) * a.tpt) : a.tpt;
+            const long long s0 = x - b.off, to = moved(x, s0, s0 + b.cost, ntok * a.group, s_plan.extra);
             b.at = to;
             b.off = int(to - s0);
             if (to == s0 + b.cost) {  // the next item
@@ -883,7 +898,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const uint32_t lane_off = uint32_t(quarter * 32) << 16;
         const int ti = row / a.group, gi = row % a.group;
         Item it;
-        Span v{0, 0, 0};
+        int row_lo = 0, row_hi = 0, row_sink = 0;  // keys that the row sees: [0, sink), [lo, hi)
         bool ok = true, valid = false, live = false;
         int k = -1;
         float m = -INFINITY, l = 0.f;  // l: this group's share, under m
@@ -898,8 +913,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 const int rows = it.ntok * a.group;
                 valid = row < rows;
                 live = quarter * 32 < rows;  // some row of the warp is there
-                v = visible(p, Request{it.tok0, it.ntok, it.len}, int64_t(it.pos0) + ti);
-                if (!valid) v = Span{0, 0, 0};
+                const Span v = visible(p, Request{it.tok0, it.ntok, it.len}, int64_t(it.pos0) + ti);
+                row_lo = int(v.lo);
+                row_hi = valid ? int(v.hi) : 0;
+                row_sink = valid ? int(v.sink) : 0;
                 m = -INFINITY;
                 l = 0.f;
             }
@@ -908,30 +925,33 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 ok = wait_bar(s_full[buf], uint32_t(j / NS) & 1u, s_abort);
                 if (!ok) break;
                 tc_fence_after();
-                float2 s[32];
                 float mx = -INFINITY;
-                const int64_t key0 = int64_t(s_unit[j % kNotes].tile) * kN;
-                // Keys [64 h, 64 h + 64) of the tile; both passes read them from tensor memory.
-                auto load = [&](int h) {
-                    tmem_ld64(tmem + uint32_t(buf * kN + h * 64) + lane_off, s);
-                    if (flags & kOpen) return;
-                    // bit c: this row sees key c of them
-                    auto below = [&](int64_t x) {
-                        const int64_t n = x - (key0 + h * 64);
-                        return n <= 0 ? uint64_t(0) : (n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1);
-                    };
-                    const uint64_t sees = (below(v.hi) & ~below(v.lo)) | below(v.sink);
-                    const uint32_t bits[2] = {uint32_t(sees), uint32_t(sees >> 32)};
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        if (!(bits[c >> 4] & (1u << (2 * (c & 15))))) s[c].x = -INFINITY;
-                        if (!(bits[c >> 4] & (2u << (2 * (c & 15))))) s[c].y = -INFINITY;
-                    }
-                };
+                const uint32_t at_s = tmem + uint32_t(buf * kN) + lane_off;
                 if (live) {
+                    if (!(flags & kOpen)) {
+                        // hidden keys' scores: -inf, in place
+                        const int key0 = s_unit[j % kNotes].tile * kN;
+#pragma unroll 1
+                        for (int h = 0; h < kN / 32; ++h) {
+                            // bit c: this row sees key c of the 32 from here on
+                            auto below = [&](int x) {
+                                const int n = x - (key0 + h * 32);
+                                return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u);
+                            };
+                            const uint32_t sees = (below(row_hi) & ~below(row_lo)) | below(row_sink);
+                            float s[32];
+                            tmem_ld32(at_s + h * 32, s);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                if (!(sees & (1u << c))) s[c] = -INFINITY;
+                            tmem_st32(at_s + h * 32, s);
+                        }
+                        tmem_wait_st();
+                    }
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        load(h);
+                        float2 s[32];
+                        tmem_ld64(at_s + h * 64, s);
                         float m0 = s[0].x, m1 = s[0].y, m2 = s[1].x, m3 = s[1].y;
 #pragma unroll
                         for (int c = 2; c < 32; c += 2) {
@@ -965,7 +985,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     float2 sum0 = make_float2(l, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        load(h);
+                        float2 s[32];
+                        tmem_ld64(at_s + h * 64, s);
                         float pk[32];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
@@ -977,7 +998,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                             pk[c] = __uint_as_float(cvt_pair<T>(x.x, x.y));
                         }
                         // over the scores that it came from
-                        tmem_st32(tmem + uint32_t(buf * kN + h * 64) + lane_off, pk);
+                        tmem_st32(at_s + h * 64, pk);
                     }
                     sum0 = add2(sum0, sum1);
                     l = sum0.x + sum0.y;
@@ -1029,7 +1050,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             }
             if (!ok) break;
             const uint32_t o_addr = tmem + S::O_COL + uint32_t(w * (HD / 2)) + lane_off;
-            if (s_poison[k % kNotes]) add_not_finite<HD, T>(a, it, v, w, o_addr);
+            if (s_poison[k % kNotes]) add_not_finite<HD, T>(a, it, Span{row_sink, row_lo, row_hi}, w, o_addr);
             const bool whole = it.u0 == 0 && it.u1 == it.units;
             if (live && whole) {
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
@@ -1091,7 +1112,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 const Plan& pl = s_plan;
                 int64_t c = (it.end * pl.ctas - 1) / pl.total;
                 const int64_t x = c * pl.total / pl.ctas;
-                if (x > it.start && moved(x, it.start, it.end, pl.near) == it.end) --c;
+                if (x > it.start && moved(x, it.start, it.end, it.ntok * a.group, pl.extra) == it.end) --c;
                 cut = Cut{it.tok0, it.ntok, it.h, int32_t(c), 1};
             }
             tc_fence_before();
