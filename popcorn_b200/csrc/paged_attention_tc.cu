@@ -328,7 +328,7 @@ __device__ __noinline__ bool wait_long(uint32_t b, uint32_t parity, volatile int
     *abort = 1;
     return false;
 }
-__device__ __forceinline__ bool wait_bar(uint64_t& bar, uint32_t parity, volatile int& abort) {
+__device__ __noinline__ bool wait_bar(uint64_t& bar, uint32_t parity, volatile int& abort) {
     const uint32_t b = smem_u32(&bar);
     if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
     return wait_long(b, parity, &abort);
@@ -505,6 +505,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         __syncthreads();
         long long run = iu - sum, run_items = ii - items, units = 0;
+#pragma unroll 1
         for (int x = 0; x < kPtThreads / 32; ++x) {
             if (x < warp) {
                 run += scan[x];
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 const uint32_t dst = smem_u32(ring) + slot * S::SLOT;
                 const int per = boxes / H;
                 mbar_expect_tx(bar, S::SLOT);
-                for (int b = 0; b < per; ++b)
+                _Pragma("unroll 1") for (int b = 0; b < per; ++b)
                     tma_load_4d(dst + b * a.box_groups * S::GROUP, map, 0, 0, 0, group[h * per + b], bar);
             }
         }
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     if (lane == 0) {
                         const bool one = it.ntok == 1;
                         mbar_expect_tx(smem_u32(&q_full), uint32_t(one ? a.group : a.group * a.tpt) * 128 * ATOMS);
-                        for (int at = 0; at < ATOMS; ++at)
+                        _Pragma("unroll 1") for (int at = 0; at < ATOMS; ++at)
                             tma_load_4d(smem_u32(sq + at * S::Q_BLOCK), one ? &map_q1 : &map_q, 0, it.h * a.group, it.tok0, at,
                                         smem_u32(&q_full));
                     }
@@ -847,7 +848,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&unit_free[j % kNotes]));
-            for (int h = 0; h < H && ok; ++h) {
+            _Pragma("unroll 1") for (int h = 0; h < H && ok; ++h) {
                 if (!(flags & (kLook << h))) continue;
                 const int64_t key0 = int64_t(tile) * kN + h * S::KEYS;
                 const int slot = (v_pos(j) + h) % NSLOT;
@@ -863,14 +864,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     unsigned char* base = ring + slot * S::SLOT + (kk >> 3) * S::GROUP + (kk & 7) * 128;
                     uint32_t any = 0;
                     if (seen) {
-#pragma unroll 8
+#pragma unroll 4
                         for (int i = 0; i < ATOMS * 8; ++i) {
                             const uint4 y = *reinterpret_cast<const uint4*>(base + (i >> 3) * 1024 + ((i + kk) & 7) * 16);
                             any |= not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w);
                         }
                     }
                     if (seen && !(any & 0x80008000u)) continue;
-#pragma unroll 8
+#pragma unroll 2
                     for (int i = 0; i < ATOMS * 8; ++i) {
                         uint4* x = reinterpret_cast<uint4*>(base + (i >> 3) * 1024 + ((i + kk) & 7) * 16);
                         uint4 y = make_uint4(0, 0, 0, 0);
