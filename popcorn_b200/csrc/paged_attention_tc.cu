@@ -146,6 +146,8 @@ __device__ __noinline__ void item_span(const TcArgs& a, const Request& rq, int m
 
 // A place in the step's order: `at`, `off` into item (r, h, mt), which starts
 // at `at - off` and counts `cost`.
+__device__ __noinline__ int64_t div64(int64_t a, int64_t b) { return a / b; }  // (one copy of a long sequence)
+
 struct Place {
     int r, h, mt, off;
     int64_t at, cost;
@@ -298,6 +300,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// One ring slot: `n` boxes of `step` bytes.
+__device__ __noinline__ void load_boxes(uint32_t dst, uint32_t bar, uint32_t bytes, const CUtensorMap* map, const int* group,
+                                        int n, uint32_t step) {
+    mbar_expect_tx(bar, bytes);
+#pragma unroll 1
+    for (int b = 0; b < n; ++b) tma_load_4d(dst + b * step, map, 0, 0, 0, group[b], bar);
+}
+
 // A from tensor memory (16-bit pairs, a row a lane), B from shared memory.
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -379,6 +389,99 @@ __device__ __noinline__ void add_not_finite(const TcArgs& a, const Item& it, con
             }
         }
     }
+}
+
+// ---- the softmax warps' rarer steps, out of their loop ----
+
+// Scores of the keys that the row does not see: -inf, in tensor memory.
+__device__ __noinline__ void hide_scores(uint32_t at, int key0, int lo, int hi, int sink) {
+#pragma unroll 1
+    for (int h = 0; h < kN / 32; ++h) {
+        // bit c: the row sees key c of the 32 from here on
+        auto below = [&](int x) {
+            const int n = x - (key0 + h * 32);
+            return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u);
+        };
+        const uint32_t sees = (below(hi) & ~below(lo)) | below(sink);
+        float s[32];
+        tmem_ld32(at + h * 32, s);
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            if (!(sees & (1u << c))) s[c] = -INFINITY;
+        tmem_st32(at + h * 32, s);
+    }
+    tmem_wait_st();
+}
+
+__device__ __noinline__ void scale_columns(uint32_t at, int columns, float f) {
+#pragma unroll 1
+    for (int c = 0; c < columns; c += 32) {
+        float o[32];
+        tmem_ld32(at + c, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] *= f;
+        tmem_st32(at + c, o);
+    }
+    tmem_wait_st();
+}
+
+// O times inv -> the output, `columns` columns of this thread's row from `dst` on. 16-byte chunks change places among
+// four neighbouring rows, so that four lanes store 64 bytes of a row. zero: rows of no key.
+template <class T>
+__device__ __noinline__ void store_rows(uint32_t at, int columns, uint16_t* dst, float inv, bool zero, int row, int rows) {
+    const int lane = threadIdx.x & 31, q = lane & 3;
+#pragma unroll 1
+    for (int cc = 0; cc < columns; cc += 32) {
+        float o[32];
+        tmem_ld32(at + cc, o);
+        uint32_t x[4][4];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e >> 2][e & 3] = zero ? 0u : cvt_pair<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+#pragma unroll
+        for (int step = 1; step <= 2; step <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i & step) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t give = q & step ? x[i][e] : x[i | step][e];
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, give, step);
+                    if (q & step) x[i][e] = got;
+                    else x[i | step][e] = got;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint16_t* to = reinterpret_cast<uint16_t*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & ~3) | i));
+            if (((row & ~3) | i) < rows)
+                *reinterpret_cast<uint4*>(to + cc + q * 8) = make_uint4(x[i][0], x[i][1], x[i][2], x[i][3]);
+        }
+    }
+}
+
+// A piece's O: [column / 4][row], neighbouring rows are neighbours.
+__device__ __noinline__ void store_piece(uint32_t at, int columns, float4* part, int rows_cap, bool valid) {
+#pragma unroll 1
+    for (int cc = 0; cc < columns; cc += 32) {
+        float o[32];
+        tmem_ld32(at + cc, o);
+        if (valid) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                part[int64_t(cc / 4 + e) * rows_cap] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+        __syncwarp();
+    }
+}
+
+// The CTA of an item's last piece.
+__device__ __noinline__ int last_cta(const TcArgs& a, const Item& it, const Plan& pl) {
+    int64_t c = div64(it.end * pl.ctas - 1, pl.total);
+    const int64_t x = div64(c * pl.total, pl.ctas);
+    if (x > it.start && moved(x, it.start, it.end, it.ntok * a.group, pl.extra) == it.end) --c;
+    return int(c);
 }
 
 template <int HD, class T>
@@ -533,7 +636,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         Place b{0, 0, 0, 0, U, 0};
         const int c = int(blockIdx.x) + warp;
         if (c < ctas) {
-            const long long x = c * U / ctas;
+            const long long x = div64(c * U, ctas);
             int lo = 0, hi = p.R;
 #pragma unroll 1
             while (hi - lo > 1) {
@@ -541,10 +644,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 if (cum[mid] <= x) lo = mid;
                 else hi = mid;
             }
-            const long long per_head = (cum[lo + 1] - cum[lo]) / p.Nkv;
+            const long long per_head = div64(cum[lo + 1] - cum[lo], p.Nkv);
             long long rem = x - cum[lo];
             b.r = lo;
-            b.h = int(rem / per_head);
+            b.h = int(div64(rem, per_head));
             rem -= b.h * per_head;
             // the item: 32 tiles at a time
             const Request rq = request(p, lo);
@@ -615,25 +718,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         return true;
     };
     const int boxes = kN / 8 / a.box_groups;  // TMA boxes of a tile
-    // Box b of H-th part h, its share of the tile: issued one by one by lane 0.
-    auto put = [&](const int* group, int pos, uint64_t* const* bars, const CUtensorMap* map) {
-        bool ok = true;
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const int q = pos + h, slot = q % NSLOT;
-            ok = wait_bar(empty[slot], (uint32_t(q / NSLOT) & 1u) ^ 1u, s_abort);
-            if (!ok) break;
-            if (lane == 0) {
-                const uint32_t bar = smem_u32(bars[h] ? bars[h] : &full[slot]);
-                const uint32_t dst = smem_u32(ring) + slot * S::SLOT;
-                const int per = boxes / H;
-                mbar_expect_tx(bar, S::SLOT);
-                _Pragma("unroll 1") for (int b = 0; b < per; ++b)
-                    tma_load_4d(dst + b * a.box_groups * S::GROUP, map, 0, 0, 0, group[h * per + b], bar);
-            }
-        }
+    // One slot's boxes, issued one by one by lane 0: `to` gets the bytes.
+    auto put = [&](const int* group, int q, uint64_t* to, const CUtensorMap* map) {
+        const int slot = q % NSLOT;
+        if (!wait_bar(empty[slot], (uint32_t(q / NSLOT) & 1u) ^ 1u, s_abort)) return false;
+        if (lane == 0)
+            load_boxes(smem_u32(ring) + slot * S::SLOT, smem_u32(to ? to : &full[slot]), S::SLOT, map, group, boxes / H,
+                       a.box_groups * S::GROUP);
         __syncwarp();
-        return ok;
+        return true;
     };
 
     if (warp == 0) {
@@ -717,8 +810,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     __syncwarp();
                     ++items;
                 }
-                uint64_t* const none[2] = {nullptr, nullptr};
-                ok = put(note.group, k_pos(j), none, &map_k);
+#pragma unroll 1
+                for (int h = 0; h < H && ok; ++h) ok = put(note.group + h * (boxes / H), k_pos(j) + h, nullptr, &map_k);
             }
         }
         if (ok) ok = wait_bar(unit_free[j % kNotes], (uint32_t(j / kNotes) & 1u) ^ 1u, s_abort);
@@ -735,11 +828,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
             const Unit& note = s_unit[j % kNotes];
             if (!ok || (note.flags & kStop)) break;
-            uint64_t* to[2] = {nullptr, nullptr};
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-                if (note.flags & (kLook << h)) to[h] = &look[looks++ % kNotes];
-            ok = put(note.group, v_pos(j), to, &map_v);
+#pragma unroll 1
+            for (int h = 0; h < H && ok; ++h)
+                ok = put(note.group + h * (boxes / H), v_pos(j) + h,
+                         note.flags & (kLook << h) ? &look[looks++ % kNotes] : nullptr, &map_v);
         }
         if (!ok) s_abort = 1;
     } else if (warp == 1) {
@@ -929,26 +1021,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 float mx = -INFINITY;
                 const uint32_t at_s = tmem + uint32_t(buf * kN) + lane_off;
                 if (live) {
-                    if (!(flags & kOpen)) {
-                        // hidden keys' scores: -inf, in place
-                        const int key0 = s_unit[j % kNotes].tile * kN;
-#pragma unroll 1
-                        for (int h = 0; h < kN / 32; ++h) {
-                            // bit c: this row sees key c of the 32 from here on
-                            auto below = [&](int x) {
-                                const int n = x - (key0 + h * 32);
-                                return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u);
-                            };
-                            const uint32_t sees = (below(row_hi) & ~below(row_lo)) | below(row_sink);
-                            float s[32];
-                            tmem_ld32(at_s + h * 32, s);
-#pragma unroll
-                            for (int c = 0; c < 32; ++c)
-                                if (!(sees & (1u << c))) s[c] = -INFINITY;
-                            tmem_st32(at_s + h * 32, s);
-                        }
-                        tmem_wait_st();
-                    }
+                    if (!(flags & kOpen))
+                        hide_scores(at_s, s_unit[j % kNotes].tile * kN, row_lo, row_hi, row_sink);
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         float2 s[32];
@@ -1010,17 +1084,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     ok = wait_bar(pv_done[(j - 1) % NS], uint32_t((j - 1) / NS) & 1u, s_abort);
                     if (!ok) break;
                     tc_fence_after();
-                    const float f = now != before && before != -INFINITY ? ex2(before - now) : 1.f;
-#pragma unroll 1
-                    for (int cc = 0; cc < HD / 32; ++cc) {
-                        float o[32];
-                        const uint32_t at = tmem + S::O_COL + uint32_t(cc * 32) + lane_off;
-                        tmem_ld32(at, o);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= f;
-                        tmem_st32(at, o);
-                    }
-                    tmem_wait_st();
+                    scale_columns(tmem + S::O_COL + lane_off, HD,
+                                  now != before && before != -INFINITY ? ex2(before - now) : 1.f);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -1054,68 +1119,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (s_poison[k % kNotes]) add_not_finite<HD, T>(a, it, Span{row_sink, row_lo, row_hi}, w, o_addr);
             const bool whole = it.u0 == 0 && it.u1 == it.units;
             if (live && whole) {
-                const float inv = L == 0.f ? 0.f : 1.0f / L;
-                // 16-byte chunks change places among four neighbouring rows, so that four lanes store 64 bytes of a row
-                const int q = lane & 3;
                 uint16_t* dst = static_cast<uint16_t*>(p.out) +
                                 ((int64_t(it.tok0) + ti) * p.Nq + it.h * a.group + gi) * HD + w * (HD / 2);
-#pragma unroll 1
-                for (int cc = 0; cc < HD / 64; ++cc) {
-                    float o[32];
-                    tmem_ld32(o_addr + cc * 32, o);
-                    uint32_t x[4][4];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        x[e >> 2][e & 3] = L == 0.f ? 0u : cvt_pair<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
-#pragma unroll
-                    for (int step = 1; step <= 2; step <<= 1) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (i & step) continue;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t give = q & step ? x[i][e] : x[i | step][e];
-                                const uint32_t got = __shfl_xor_sync(0xffffffffu, give, step);
-                                if (q & step) x[i][e] = got;
-                                else x[i | step][e] = got;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint16_t* to = reinterpret_cast<uint16_t*>(
-                            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & ~3) | i));
-                        if (((row & ~3) | i) < it.ntok * a.group)
-                            *reinterpret_cast<uint4*>(to + cc * 32 + q * 8) = make_uint4(x[i][0], x[i][1], x[i][2], x[i][3]);
-                    }
-                }
+                store_rows<T>(o_addr, HD / 2, dst, L == 0.f ? 0.f : 1.0f / L, L == 0.f, row, it.ntok * a.group);
             } else if (live) {
                 const int64_t slot = 2 * int64_t(blockIdx.x) + (it.u0 > 0 ? 0 : 1);
-                // [column / 4][row]: neighbouring rows are neighbours
-                float4* part = reinterpret_cast<float4*>(a.po) + (slot * (HD / 4) + w * (HD / 8)) * a.rows_cap + row;
-#pragma unroll 1
-                for (int cc = 0; cc < HD / 64; ++cc) {
-                    float o[32];
-                    tmem_ld32(o_addr + cc * 32, o);
-                    if (valid) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            part[(cc * 8 + e) * a.rows_cap] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                    }
-                    __syncwarp();
-                }
+                store_piece(o_addr, HD / 2,
+                            reinterpret_cast<float4*>(a.po) + (slot * (HD / 4) + w * (HD / 8)) * a.rows_cap + row, a.rows_cap,
+                            valid);
                 if (valid && w == 0) {
                     a.pml[slot * 2 * a.rows_cap + row] = last_m;
                     a.pml[(slot * 2 + 1) * a.rows_cap + row] = L;
                 }
             }
-            if (it.u0 == 0 && !whole && warp == 4) {
-                const Plan& pl = s_plan;
-                int64_t c = (it.end * pl.ctas - 1) / pl.total;
-                const int64_t x = c * pl.total / pl.ctas;
-                if (x > it.start && moved(x, it.start, it.end, it.ntok * a.group, pl.extra) == it.end) --c;
-                cut = Cut{it.tok0, it.ntok, it.h, int32_t(c), 1};
-            }
+            if (it.u0 == 0 && !whole && warp == 4) cut = Cut{it.tok0, it.ntok, it.h, last_cta(a, it, s_plan), 1};
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&o_free));
