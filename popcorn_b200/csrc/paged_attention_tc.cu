@@ -17,8 +17,9 @@
 // In a CTA: warp 0 walks the items, looks pages up and loads Q and K by TMA
 // (128-byte swizzle, a box per run of page rows); warp 2 loads V; both fill
 // one ring in the order K(0), K(1), V(0), K(2), V(1), ...; warp 1 issues S = Q.K^T
-// into the next of NS accumulators in tensor memory and O += P.V, whichever
-// is ready; warps 4-7 and 8-11 take tiles in turn (a thread a row) and turn S
+// into the next of NS accumulators in tensor memory, warp 12 O += P.V (one
+// issuer for both spent half of its time in looking at barriers, some 150
+// clocks each: 2430 instead of 1700 clocks a tile at Hd 128); warps 4-7 and 8-11 take tiles in turn (a thread a row) and turn S
 // into P = 2^(c S - m): P is packed into the type and written back over S,
 // from where the second product reads it as its A operand, so it never passes
 // through shared memory; one group's loads and waits pass under the other's
@@ -60,7 +61,7 @@ using namespace tc;
 
 constexpr int kM = 128;          // query rows of an item
 constexpr int kN = 128;          // keys of a unit
-constexpr int kPtThreads = 384;  // warps: 0 Q and K loads, 1 MMA, 2 V loads, 3 masked V, 4-11 softmax
+constexpr int kPtThreads = 416;  // warps: 0 Q and K loads, 1 Q.K^T, 2 V loads, 3 masked V, 4-11 softmax, 12 P.V
 constexpr int kSoftWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 of the growth of a row's max that is let pass
@@ -123,29 +124,54 @@ struct Item {
     int64_t start, end;   // where the item lies in the step's order
 };
 
+// A request and a row's keys in 32 bits (every length is at most 2^30 here): [0, sink) and [lo, hi).
+struct Req {
+    int t0, n, len;
+};
+__device__ __forceinline__ Req req(const PagedAttention& p, int r) {
+    int a = p.query_start[r], b = p.query_start[r + 1], len = p.seq_lens[r];
+    const int T = int(p.T), most = int(p.W * p.ps);
+    a = a < 0 ? 0 : (a > T ? T : a);
+    b = b < a ? a : (b > T ? T : b);
+    len = len < 0 ? 0 : (len > most ? most : len);
+    return Req{a, b - a, len};
+}
+struct Keys {
+    int sink, lo, hi;
+};
+__device__ __forceinline__ Keys keys_of(const PagedAttention& p, int len, int pos) {
+    Keys v{0, 0, len};
+    if (p.mask_kind != 2) v.hi = pos < 0 ? 0 : (pos < len ? pos + 1 : len);
+    if (p.mask_kind == 1) {
+        v.lo = pos >= p.window ? pos - p.window + 1 : 0;
+        if (v.lo > v.hi) v.lo = v.hi;
+        v.sink = p.sinks < v.lo ? p.sinks : v.lo;
+    }
+    return v;
+}
+
 // (Not inlined: the roles' loops are long, and the instruction cache is what they share.)
-__device__ __noinline__ void item_span(const TcArgs& a, const Request& rq, int mt, Item& it) {
+__device__ __noinline__ void item_span(const TcArgs& a, const Req& rq, int mt, Item& it) {
     const PagedAttention& p = a.p;
-    const int64_t i0 = int64_t(mt) * a.tpt;
-    it.tok0 = int(rq.t0 + i0);
-    it.ntok = int(rq.n - i0 < a.tpt ? rq.n - i0 : a.tpt);
-    const int64_t pos0 = rq.len - rq.n + i0;
-    it.pos0 = int(pos0);
-    it.len = int(rq.len);
-    const Span first = visible(p, rq, pos0), last = visible(p, rq, pos0 + it.ntok - 1);
-    it.lo = int(first.lo);
-    it.hi = int(last.hi);
-    it.sink = int(last.sink);
+    const int i0 = mt * a.tpt;
+    it.tok0 = rq.t0 + i0;
+    it.ntok = rq.n - i0 < a.tpt ? rq.n - i0 : a.tpt;
+    it.pos0 = rq.len - rq.n + i0;
+    it.len = rq.len;
+    const Keys first = keys_of(p, rq.len, it.pos0), last = keys_of(p, rq.len, it.pos0 + it.ntok - 1);
+    it.lo = first.lo;
+    it.hi = last.hi;
+    it.sink = last.sink;
     it.t_lo = it.lo / kN;
-    const int t_hi = int((last.hi + kN - 1) / kN);
-    const int ns = int((last.sink + kN - 1) / kN);
+    const int t_hi = (last.hi + kN - 1) / kN, ns = (last.sink + kN - 1) / kN;
     it.ns = ns < it.t_lo ? ns : it.t_lo;
     const int u = it.ns + (t_hi > it.t_lo ? t_hi - it.t_lo : 0);
     it.units = u > 1 ? u : 1;  // (rows without a key are written too)
 }
+__device__ __forceinline__ int tiles_of(const TcArgs& a, const Req& rq) {
+    return int(unsigned(rq.n + a.tpt - 1) / unsigned(a.tpt));
+}
 
-// A place in the step's order: `at`, `off` into item (r, h, mt), which starts
-// at `at - off` and counts `cost`.
 __device__ __noinline__ int64_t div64(int64_t a, int64_t b) { return a / b; }  // (one copy of a long sequence)
 
 struct Place {
@@ -170,7 +196,7 @@ __device__ __forceinline__ int64_t moved(int64_t x, int64_t s, int64_t e, int ro
 // The CTA's items in order (walked by warp 0, which tells the others).
 struct Walk {
     const TcArgs& a;
-    Request rq;
+    Req rq;
     int r, h, mt, off, ntiles, extra;
     int64_t at, end;
 
@@ -179,8 +205,8 @@ struct Walk {
         if (at < end) load();
     }
     __device__ __forceinline__ void load() {
-        rq = request(a.p, r);
-        ntiles = int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt));
+        rq = req(a.p, r);
+        ntiles = tiles_of(a, rq);
     }
     __device__ __noinline__ bool next(Item& it) {
         while (at < end) {
@@ -201,7 +227,7 @@ struct Walk {
                     h = 0;
                     if (at < end) {
                         do ++r;
-                        while (r < a.p.R && request(a.p, r).n == 0);
+                        while (r < a.p.R && req(a.p, r).n == 0);
                         if (r < a.p.R) load();
                         else at = end;
                     }
@@ -216,19 +242,19 @@ struct Walk {
 __device__ __forceinline__ int tile_of(const Item& it, int u) { return u < it.ns ? u : it.t_lo + (u - it.ns); }
 
 // Every row of the item sees every one of the `keys` keys from key0 on.
-__device__ __forceinline__ bool keys_open(const TcArgs& a, const Item& it, int64_t key0, int keys) {
+__device__ __forceinline__ bool keys_open(const TcArgs& a, const Item& it, int key0, int keys) {
     const PagedAttention& p = a.p;
-    const int64_t end = p.mask_kind == 2 ? it.len : (int64_t(it.pos0) + 1 < it.len ? int64_t(it.pos0) + 1 : it.len);
+    const int end = p.mask_kind == 2 ? it.len : (it.pos0 < it.len ? it.pos0 + 1 : it.len);
     if (key0 + keys > end) return false;
     if (p.mask_kind != 1) return true;
-    return key0 >= int64_t(it.pos0) + it.ntok - p.window || key0 + keys <= p.sinks;
+    return key0 > it.pos0 + it.ntok - 1 - p.window || key0 + keys <= p.sinks;
 }
 // Some row of the item sees one of them.
-__device__ __forceinline__ bool keys_seen(const Item& it, int64_t key0, int keys) {
+__device__ __forceinline__ bool keys_seen(const Item& it, int key0, int keys) {
     return key0 < it.hi && (key0 + keys > it.lo || key0 < it.sink);
 }
 // The V rows of a slot of `keys` keys need a look before the product reads them.
-__device__ __forceinline__ bool guarded(const TcArgs& a, const Item& it, int64_t key0, int keys) {
+__device__ __forceinline__ bool guarded(const TcArgs& a, const Item& it, int key0, int keys) {
     return keys_seen(it, key0, keys) && !keys_open(a, it, key0, keys);
 }
 
@@ -237,7 +263,8 @@ enum : int {
     kFirst = 1, kLast = 2,  // of its item in this CTA
     kOpen = 4,              // every row sees every key of the tile
     kStop = 8,              // no unit: the CTA is done
-    kLook = 16              // kLook << h: half h of V is guarded
+    kNextFirst = 16, kNextLast = 32, kNextStop = 64,  // the same of the unit after it
+    kLook = 128             // kLook << h: half h of V is guarded
 };
 struct Unit {
     int flags;
@@ -344,6 +371,28 @@ __device__ __noinline__ bool wait_bar(uint64_t& bar, uint32_t parity, volatile i
     return wait_long(b, parity, &abort);
 }
 
+// The same, its first look in line: for the softmax warps' turns.
+__device__ __forceinline__ bool wait_fast(uint64_t& bar, uint32_t parity, volatile int& abort) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&bar), parity))) return true;
+    return wait_long(smem_u32(&bar), parity, &abort);
+}
+
+// The same for one thread.
+__device__ __noinline__ bool wait_one_long(uint32_t b, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+    for (int i = 0; i < 20000; ++i) {
+        if (mbar_try_wait(b, parity)) return true;
+        if (*abort) return false;
+    }
+    atomicOr(&g_pt_error_word, 1u);
+    *abort = 1;
+    return false;
+}
+__device__ __forceinline__ bool wait_one(uint64_t& bar, uint32_t parity, volatile int& abort) {
+    const uint32_t b = smem_u32(&bar);
+    return mbar_try_wait(b, parity) || wait_one_long(b, parity, &abort);
+}
+
 // Exponent fields of two 16-bit values: bit 15 of a half is set in the result where its value is not finite.
 template <class T>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
@@ -357,22 +406,184 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
     return w & ~((bad >> 15) * 0xffffu);
 }
 
+// The plan: sums of the requests' units, and where this CTA's run begins and ends. cum [R + 1] and scan [2 * warps] are
+// shared memory that no copy uses yet. Every thread of the CTA calls it.
+__device__ __noinline__ void make_plan(const TcArgs& a, long long* cum, long long* scan, Plan& plan) {
+    const PagedAttention& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto head_units = [&](const Req& rq, int from, int step) {
+        long long u = 0;
+        const int nt = tiles_of(a, rq);
+        Item it;
+#pragma unroll 1
+        for (int mt = from; mt < nt; mt += step) {
+            item_span(a, rq, mt, it);
+            u += it.units;
+        }
+        return u;
+    };
+    // a thread a request; one of many tiles is left to a warp
+    constexpr int kFewTiles = 4;
+    int many = 0;
+#pragma unroll 1
+    for (int r = tid; r < p.R; r += kPtThreads) {
+        const Req rq = req(p, r);
+        const bool few = tiles_of(a, rq) <= kFewTiles;
+        cum[r + 1] = few ? head_units(rq, 0, 1) * p.Nkv : -1;
+        many |= !few;
+    }
+    if (__syncthreads_or(many)) {
+#pragma unroll 1
+        for (int r = warp; r < p.R; r += kPtThreads / 32) {
+            if (cum[r + 1] >= 0) continue;
+            long long u = head_units(req(p, r), lane, 32);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+            __syncwarp();
+            if (lane == 0) cum[r + 1] = u * p.Nkv;
+        }
+    }
+    if (tid == 0) cum[0] = 0;
+    __syncthreads();
+    {
+        // each thread sums a run of requests, units and items
+        const int per = (p.R + kPtThreads - 1) / kPtThreads;
+        const int r0 = tid * per < p.R ? tid * per : p.R, r1 = r0 + per < p.R ? r0 + per : p.R;
+        long long sum = 0, items = 0;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            sum += cum[r + 1];
+            items += (long long)tiles_of(a, req(p, r)) * p.Nkv;
+        }
+        long long iu = sum, ii = items;  // inclusive over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, iu, o), y = __shfl_up_sync(0xffffffffu, ii, o);
+            if (lane >= o) {
+                iu += x;
+                ii += y;
+            }
+        }
+        if (lane == 31) {
+            scan[warp] = iu;
+            scan[kPtThreads / 32 + warp] = ii;
+        }
+        __syncthreads();
+        long long run = iu - sum, run_items = ii - items, units = 0;
+#pragma unroll 1
+        for (int x = 0; x < kPtThreads / 32; ++x) {
+            if (x < warp) {
+                run += scan[x];
+                run_items += scan[kPtThreads / 32 + x];
+            }
+            units += scan[x];
+        }
+        // With runs long enough, an item counts for its epilogue too, and cuts keep clear of its ends.
+        const int extra = units >= 16ll * gridDim.x ? 1 : 0;
+        run += extra * run_items;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            run += cum[r + 1] + (extra ? (long long)tiles_of(a, req(p, r)) * p.Nkv : 0);
+            cum[r + 1] = run;
+        }
+        if (tid == 0) {
+            plan.extra = extra;
+        }
+    }
+    __syncthreads();
+    if (warp < 2) {
+        // warp 0: where the run begins, warp 1: where it ends
+        const long long U = cum[p.R];
+        const int ctas = U < (long long)gridDim.x ? int(U) : int(gridDim.x);
+        Place b{0, 0, 0, 0, U, 0};
+        const int c = int(blockIdx.x) + warp;
+        if (c < ctas) {
+            const long long x = div64(c * U, ctas);
+            int lo = 0, hi = p.R;
+#pragma unroll 1
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (cum[mid] <= x) lo = mid;
+                else hi = mid;
+            }
+            const long long per_head = div64(cum[lo + 1] - cum[lo], p.Nkv);
+            long long rem = x - cum[lo];
+            b.r = lo;
+            b.h = int(div64(rem, per_head));
+            rem -= b.h * per_head;
+            // the item: 32 tiles at a time
+            const Req rq = req(p, lo);
+            const int nt = tiles_of(a, rq);
+#pragma unroll 1
+            for (int mt0 = 0; mt0 < nt; mt0 += 32) {
+                Item it;
+                it.units = 0;
+                if (mt0 + lane < nt) {
+                    item_span(a, rq, mt0 + lane, it);
+                    it.units += plan.extra;
+                }
+                long long incl = it.units;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += y;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, incl > rem);
+                if (hit) {
+                    const int l = __ffs(int(hit)) - 1;
+                    b.mt = mt0 + l;
+                    b.off = int(rem - __shfl_sync(0xffffffffu, incl - it.units, l));
+                    b.cost = __shfl_sync(0xffffffffu, it.units, l);
+                    break;
+                }
+                rem -= __shfl_sync(0xffffffffu, incl, 31);
+            }
+            const int ntok = rq.n - b.mt * a.tpt < a.tpt ? rq.n - b.mt * a.tpt : a.tpt;
+            const long long s0 = x - b.off, to = moved(x, s0, s0 + b.cost, ntok * a.group, plan.extra);
+            b.at = to;
+            b.off = int(to - s0);
+            if (to == s0 + b.cost) {  // the next item
+                b.off = 0;
+                if (++b.mt == nt) {
+                    b.mt = 0;
+                    if (++b.h == p.Nkv) {
+                        b.h = 0;
+#pragma unroll 1
+                        do ++b.r;
+                        while (b.r < p.R && req(p, b.r).n == 0);
+                    }
+                }
+            }
+        }
+        if (lane == 0) {
+            if (warp == 0) {
+                plan.begin = b;
+                plan.total = U;
+                plan.ctas = ctas;
+            } else {
+                plan.end = b.at;
+            }
+        }
+    }
+}
+
 // The product left out V values that are not finite, in slots where some row does not see some key: adds them to the
 // rows that see them (an infinity or a NaN outweighs any weight). O's columns [w Hd / 2, (w + 1) Hd / 2) are at `o_addr`.
 template <int HD, class T>
-__device__ __noinline__ void add_not_finite(const TcArgs& a, const Item& it, const Span& v, int w, uint32_t o_addr) {
+__device__ __noinline__ void add_not_finite(const TcArgs& a, const Item& it, const Keys& v, int w, uint32_t o_addr) {
     const PagedAttention& p = a.p;
     constexpr int KEYS = Shape<HD>::KEYS;
 #pragma unroll 1
     for (int x = it.u0; x < it.u1; ++x) {
-        const int64_t key0 = int64_t(tile_of(it, x)) * kN;
+        const int key0 = tile_of(it, x) * kN;
 #pragma unroll 1
-        for (int64_t key = key0; key < key0 + kN; ++key) {
-            if (!keys_seen(it, key, 1) || !guarded(a, it, key & ~int64_t(KEYS - 1), KEYS)) continue;
-            const int32_t page = p.table[int64_t(it.r) * p.W + key / p.ps];
+        for (int key = key0; key < key0 + kN; ++key) {
+            if (!keys_seen(it, key, 1) || !guarded(a, it, key & ~(KEYS - 1), KEYS)) continue;
+            const uint32_t ps = uint32_t(p.ps);
+            const int32_t page = p.table[int64_t(it.r) * p.W + uint32_t(key) / ps];
             if (page < 0 || page >= p.P) continue;
             const bool sees = (key >= v.lo && key < v.hi) || key < v.sink;
-            const int64_t vrow = ((int64_t(page) * p.Nkv + it.h) * p.ps + key % p.ps) * HD + w * (HD / 2);
+            const int64_t vrow = ((int64_t(page) * p.Nkv + it.h) * p.ps + uint32_t(key) % ps) * HD + w * (HD / 2);
 #pragma unroll 1
             for (int cc = 0; cc < HD / 64; ++cc) {
                 const float mine = Elem<T>::load(p.v_pages, vrow + cc * 32 + (threadIdx.x & 31));
@@ -545,164 +756,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), kTmem);
     pdl_wait();
 
-    // ---- the plan: sums of the requests' units, and where this CTA's run begins and ends ----
-    long long* cum = reinterpret_cast<long long*>(ring);  // [R + 1], before any copy uses the ring
-    long long* scan = reinterpret_cast<long long*>(sq);   // [2 * warps]
-    auto tiles_of = [&](const Request& rq) { return int((unsigned(rq.n) + unsigned(a.tpt) - 1) / unsigned(a.tpt)); };
-    auto head_units = [&](const Request& rq, int from, int step) {
-        long long u = 0;
-        const int nt = tiles_of(rq);
-        Item it;
-#pragma unroll 1
-        for (int mt = from; mt < nt; mt += step) {
-            item_span(a, rq, mt, it);
-            u += it.units;
-        }
-        return u;
-    };
-    // a thread a request; one of many tiles is left to a warp
-    constexpr int kFewTiles = 4;
-    int many = 0;
-#pragma unroll 1
-    for (int r = tid; r < p.R; r += kPtThreads) {
-        const Request rq = request(p, r);
-        const bool few = tiles_of(rq) <= kFewTiles;
-        cum[r + 1] = few ? head_units(rq, 0, 1) * p.Nkv : -1;
-        many |= !few;
-    }
-    if (__syncthreads_or(many)) {
-#pragma unroll 1
-        for (int r = warp; r < p.R; r += kPtThreads / 32) {
-            if (cum[r + 1] >= 0) continue;
-            long long u = head_units(request(p, r), lane, 32);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-            __syncwarp();
-            if (lane == 0) cum[r + 1] = u * p.Nkv;
-        }
-    }
-    if (tid == 0) cum[0] = 0;
-    __syncthreads();
-    {
-        // each thread sums a run of requests, units and items
-        const int per = (p.R + kPtThreads - 1) / kPtThreads;
-        const int r0 = tid * per < p.R ? tid * per : p.R, r1 = r0 + per < p.R ? r0 + per : p.R;
-        long long sum = 0, items = 0;
-#pragma unroll 1
-        for (int r = r0; r < r1; ++r) {
-            sum += cum[r + 1];
-            items += (long long)tiles_of(request(p, r)) * p.Nkv;
-        }
-        long long iu = sum, ii = items;  // inclusive over the warp
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, iu, o), y = __shfl_up_sync(0xffffffffu, ii, o);
-            if (lane >= o) {
-                iu += x;
-                ii += y;
-            }
-        }
-        if (lane == 31) {
-            scan[warp] = iu;
-            scan[kPtThreads / 32 + warp] = ii;
-        }
-        __syncthreads();
-        long long run = iu - sum, run_items = ii - items, units = 0;
-#pragma unroll 1
-        for (int x = 0; x < kPtThreads / 32; ++x) {
-            if (x < warp) {
-                run += scan[x];
-                run_items += scan[kPtThreads / 32 + x];
-            }
-            units += scan[x];
-        }
-        // With runs long enough, an item counts for its epilogue too, and cuts keep clear of its ends.
-        const int extra = units >= 16ll * gridDim.x ? 1 : 0;
-        run += extra * run_items;
-#pragma unroll 1
-        for (int r = r0; r < r1; ++r) {
-            run += cum[r + 1] + (extra ? (long long)tiles_of(request(p, r)) * p.Nkv : 0);
-            cum[r + 1] = run;
-        }
-        if (tid == 0) {
-            s_plan.extra = extra;
-        }
-    }
-    __syncthreads();
-    if (warp < 2) {
-        // warp 0: where the run begins, warp 1: where it ends
-        const long long U = cum[p.R];
-        const int ctas = U < (long long)gridDim.x ? int(U) : int(gridDim.x);
-        Place b{0, 0, 0, 0, U, 0};
-        const int c = int(blockIdx.x) + warp;
-        if (c < ctas) {
-            const long long x = div64(c * U, ctas);
-            int lo = 0, hi = p.R;
-#pragma unroll 1
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (cum[mid] <= x) lo = mid;
-                else hi = mid;
-            }
-            const long long per_head = div64(cum[lo + 1] - cum[lo], p.Nkv);
-            long long rem = x - cum[lo];
-            b.r = lo;
-            b.h = int(div64(rem, per_head));
-            rem -= b.h * per_head;
-            // the item: 32 tiles at a time
-            const Request rq = request(p, lo);
-            const int nt = tiles_of(rq);
-#pragma unroll 1
-            for (int mt0 = 0; mt0 < nt; mt0 += 32) {
-                Item it;
-                it.units = 0;
-                if (mt0 + lane < nt) {
-                    item_span(a, rq, mt0 + lane, it);
-                    it.units += s_plan.extra;
-                }
-                long long incl = it.units;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += y;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, incl > rem);
-                if (hit) {
-                    const int l = __ffs(int(hit)) - 1;
-                    b.mt = mt0 + l;
-                    b.off = int(rem - __shfl_sync(0xffffffffu, incl - it.units, l));
-                    b.cost = __shfl_sync(0xffffffffu, it.units, l);
-                    break;
-                }
-                rem -= __shfl_sync(0xffffffffu, incl, 31);
-            }
-            const int ntok = rq.n - int64_t(b.mt) * a.tpt < a.tpt ? int(rq.n - int64_t(b.mt) * a.tpt) : a.tpt;
-            const long long s0 = x - b.off, to = moved(x, s0, s0 + b.cost, ntok * a.group, s_plan.extra);
-            b.at = to;
-            b.off = int(to - s0);
-            if (to == s0 + b.cost) {  // the next item
-                b.off = 0;
-                if (++b.mt == nt) {
-                    b.mt = 0;
-                    if (++b.h == p.Nkv) {
-                        b.h = 0;
-#pragma unroll 1
-                        do ++b.r;
-                        while (b.r < p.R && request(p, b.r).n == 0);
-                    }
-                }
-            }
-        }
-        if (lane == 0) {
-            if (warp == 0) {
-                s_plan.begin = b;
-                s_plan.total = U;
-                s_plan.ctas = ctas;
-            } else {
-                s_plan.end = b.at;
-            }
-        }
-    }
+    make_plan(a, reinterpret_cast<long long*>(ring), reinterpret_cast<long long*>(sq), s_plan);
     tc_fence_before();
     fence_async_smem();  // the sums' readers are done before copies land there
     __syncthreads();
@@ -740,7 +794,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         // latency is longer than a tile's loads take to issue.
         auto page_of = [&](const Item& t, int u) {
             if (u + my_unit >= t.u1) return -1;
-            const int64_t k0 = int64_t(tile_of(t, u + my_unit)) * kN + my_box * box_keys;
+            const int k0 = tile_of(t, u + my_unit) * kN + my_box * box_keys;
             if (!keys_seen(t, k0, box_keys)) return -1;
             const int32_t page = p.table[int64_t(t.r) * p.W + int64_t(__umul64hi(uint64_t(k0), a.ps_inv))];
             return page >= 0 ? page : 0x7fffffff;
@@ -781,9 +835,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 if (my_unit == u - u_first) note.group[my_box] = g;
                 __syncwarp();
                 if (lane == 0) {
-                    const int64_t key0 = int64_t(tile_of(it, u)) * kN;
+                    const int key0 = tile_of(it, u) * kN;
                     int flags = (u == it.u0 ? kFirst : 0) | (u == it.u1 - 1 ? kLast : 0) |
                                 (keys_open(a, it, key0, kN) ? kOpen : 0);
+                    if (u + 1 < it.u1) flags |= u + 2 == it.u1 ? kNextLast : 0;
+                    else flags |= !more ? kNextStop : (kNextFirst | (nx.u0 + 1 == nx.u1 ? kNextLast : 0));
                     note.tile = tile_of(it, u);
 #pragma unroll
                     for (int h = 0; h < H; ++h)
@@ -835,93 +891,81 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (!ok) s_abort = 1;
     } else if (warp == 1) {
+        // ---- S = Q.K^T ----
         if (lane == 0) {
-            // ---- MMA issue ----
             constexpr uint32_t idesc_s = make_idesc(BF, kM, kN, false), idesc_h = make_idesc(BF, kM, kN / 2, false);
-            constexpr uint32_t idesc_o = make_idesc(BF, kM, HD, true);
             const uint32_t q_base = smem_u32(sq), ring_a = smem_u32(ring);
-            auto is_full = [&](int q) {
-                return mbar_test_wait(smem_u32(&full[q % NSLOT]), uint32_t(q / NSLOT) & 1u);
-            };
-            int ns = 0, np = 0;  // next tile of S, of O
-            int ks = 0, kp = 0;  // their items
-            int fs = 0;          // the notes on tile ns (0: not read yet)
-            bool ok = true, stop = false;
-            uint32_t idle = 0;
-            while (!(stop && np == ns) && !s_abort) {
-                bool progressed = false;
-                if (!stop && ns < np + NS) {
-                    const int buf = ns % NS;
-                    const int q0 = k_pos(ns), q1 = q0 + H - 1;
-                    if (fs == 0 && mbar_test_wait(smem_u32(&unit_full[ns % kNotes]), uint32_t(ns / kNotes) & 1u))
-                        fs = s_unit[ns % kNotes].flags | 256;
-                    stop = fs & kStop;
-                    if (fs && !stop && (ns < NS || mbar_test_wait(smem_u32(&pv_done[buf]), uint32_t(ns / NS - 1) & 1u)) &&
-                        (!(fs & kFirst) || mbar_test_wait(smem_u32(&q_full), uint32_t(ks) & 1u)) && is_full(q0) &&
-                        (H == 1 || is_full(q1))) {
-                        tc_fence_after();
-                        const int s0 = q0 % NSLOT, s1 = q1 % NSLOT;
-                        const uint32_t k0 = ring_a + s0 * S::SLOT, k1 = ring_a + s1 * S::SLOT;
-                        const uint32_t d = tmem + uint32_t(buf * kN);
-                        // one N = 128 product, or two of 64 where the tile wraps round the ring
-                        const bool one = H == 1 || s1 == s0 + 1;
+            bool ok = true;
+            for (int j = 0, k = 0; ok; ++j) {
+                const int buf = j % NS;
+                ok = wait_one(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
+                const int flags = s_unit[j % kNotes].flags;
+                if (!ok || (flags & kStop)) break;
+                const int q0 = k_pos(j), q1 = q0 + H - 1;
+                const int s0 = q0 % NSLOT, s1 = q1 % NSLOT;
+                if (flags & kFirst) ok = wait_one(q_full, uint32_t(k++) & 1u, s_abort);
+                if (ok && j >= NS) ok = wait_one(pv_done[buf], uint32_t(j / NS - 1) & 1u, s_abort);
+                if (ok) ok = wait_one(full[s0], uint32_t(q0 / NSLOT) & 1u, s_abort);
+                if (ok && H > 1) ok = wait_one(full[s1], uint32_t(q1 / NSLOT) & 1u, s_abort);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t k0 = ring_a + s0 * S::SLOT, k1 = ring_a + s1 * S::SLOT;
+                const uint32_t d = tmem + uint32_t(buf * kN);
+                // one N = 128 product, or two of 64 where the tile wraps round the ring
+                const bool one = H == 1 || s1 == s0 + 1;
 #pragma unroll 1
-                        for (int h = 0; h < (one ? 1 : 2); ++h) {
-                            uint64_t da = smem_desc_sw128(q_base), db = desc_k(h ? k1 : k0, S::GROUP);
-                            const uint32_t to = d + uint32_t(h * (kN / 2)), idesc = one ? idesc_s : idesc_h;
+                for (int h = 0; h < (one ? 1 : 2); ++h) {
+                    uint64_t da = smem_desc_sw128(q_base), db = desc_k(h ? k1 : k0, S::GROUP);
+                    const uint32_t to = d + uint32_t(h * (kN / 2)), idesc = one ? idesc_s : idesc_h;
 #pragma unroll 1
-                            for (int at = 0; at < ATOMS; ++at) {
+                    for (int at = 0; at < ATOMS; ++at) {
 #pragma unroll
-                                for (int kk = 0; kk < 4; ++kk) tc_mma(to, da + 2 * kk, db + 2 * kk, idesc, (at | kk) ? 1u : 0u);
-                                da += S::Q_BLOCK >> 4;
-                                db += 1024 >> 4;
-                            }
-                        }
-                        tc_commit(smem_u32(&empty[s0]));
-                        if (H > 1) tc_commit(smem_u32(&empty[s1]));
-                        tc_commit(smem_u32(&s_full[buf]));
-                        if (fs & kFirst) ++ks;
-                        if (fs & kLast) tc_commit(smem_u32(&q_empty));
-                        fs = 0;
-                        ++ns;
-                        progressed = true;
+                        for (int kk = 0; kk < 4; ++kk) tc_mma(to, da + 2 * kk, db + 2 * kk, idesc, (at | kk) ? 1u : 0u);
+                        da += S::Q_BLOCK >> 4;
+                        db += 1024 >> 4;
                     }
                 }
-                if (np < ns) {
-                    const int buf = np % NS;
-                    const int q0 = v_pos(np), q1 = q0 + H - 1;
-                    const int fp = s_unit[np % kNotes].flags;
-                    const bool first = fp & kFirst;
-                    if (mbar_test_wait(smem_u32(&p_full[buf]), uint32_t(np / NS) & 1u) && is_full(q0) &&
-                        (H == 1 || is_full(q1)) &&
-                        (!first || kp == 0 || mbar_test_wait(smem_u32(&o_free), uint32_t(kp - 1) & 1u))) {
-                        tc_fence_after();
-                        const int s0 = q0 % NSLOT, s1 = q1 % NSLOT;
-                        const uint32_t pa = tmem + uint32_t(buf * kN);
+                tc_commit(smem_u32(&s_full[buf]));
+                tc_commit(smem_u32(&empty[s0]));
+                if (H > 1) tc_commit(smem_u32(&empty[s1]));
+                if (flags & kLast) tc_commit(smem_u32(&q_empty));
+            }
+            if (!ok) s_abort = 1;
+        }
+    } else if (warp == 12) {
+        // ---- O += P.V ----
+        if (lane == 0) {
+            constexpr uint32_t idesc_o = make_idesc(BF, kM, HD, true);
+            const uint32_t ring_a = smem_u32(ring);
+            bool ok = true;
+            for (int j = 0, k = 0; ok; ++j) {
+                const int buf = j % NS;
+                ok = wait_one(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
+                const int flags = s_unit[j % kNotes].flags;
+                if (!ok || (flags & kStop)) break;
+                const int q0 = v_pos(j), q1 = q0 + H - 1;
+                const int s0 = q0 % NSLOT, s1 = q1 % NSLOT;
+                const bool first = flags & kFirst;
+                if (first && k++ > 0) ok = wait_one(o_free, uint32_t(k - 2) & 1u, s_abort);
+                // (P(j) first: with it K(j) has landed, which had V(j)'s slot before it at Hd 256)
+                if (ok) ok = wait_one(p_full[buf], uint32_t(j / NS) & 1u, s_abort);
+                if (ok) ok = wait_one(full[s0], uint32_t(q0 / NSLOT) & 1u, s_abort);
+                if (ok && H > 1) ok = wait_one(full[s1], uint32_t(q1 / NSLOT) & 1u, s_abort);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t pa = tmem + uint32_t(buf * kN);
 #pragma unroll 1
-                        for (int h = 0; h < 2; ++h) {  // 64 keys each
-                            const uint32_t v = ring_a + (H == 1 ? s0 * S::SLOT + h * (S::SLOT / 2) : (h ? s1 : s0) * S::SLOT);
-                            const uint64_t db = desc_mn(v, S::GROUP);
+                for (int h = 0; h < 2; ++h) {  // 64 keys each
+                    const uint32_t v = ring_a + (H == 1 ? s0 * S::SLOT + h * (S::SLOT / 2) : (h ? s1 : s0) * S::SLOT);
+                    const uint64_t db = desc_mn(v, S::GROUP);
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-                                tc_mma_ts(tmem + S::O_COL, pa + h * 64 + kk * 8, db + uint64_t(kk * (2 * S::GROUP >> 4)), idesc_o,
-                                          (!first || h > 0 || kk > 0) ? 1u : 0u);
-                        }
-                        tc_commit(smem_u32(&empty[s0]));
-                        if (H > 1) tc_commit(smem_u32(&empty[s1]));
-                        tc_commit(smem_u32(&pv_done[buf]));
-                        if (first) ++kp;
-                        ++np;
-                        progressed = true;
-                    }
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc_mma_ts(tmem + S::O_COL, pa + h * 64 + kk * 8, db + uint64_t(kk * (2 * S::GROUP >> 4)), idesc_o,
+                                  (!first || h > 0 || kk > 0) ? 1u : 0u);
                 }
-                if (progressed) {
-                    idle = 0;
-                } else if (++idle > (1u << 26)) {
-                    atomicOr(&g_pt_error_word, 1u);
-                    ok = false;
-                    break;
-                }
+                tc_commit(smem_u32(&pv_done[buf]));
+                tc_commit(smem_u32(&empty[s0]));
+                if (H > 1) tc_commit(smem_u32(&empty[s1]));
             }
             if (!ok) s_abort = 1;
         }
@@ -942,7 +986,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (lane == 0) mbar_arrive(smem_u32(&unit_free[j % kNotes]));
             _Pragma("unroll 1") for (int h = 0; h < H && ok; ++h) {
                 if (!(flags & (kLook << h))) continue;
-                const int64_t key0 = int64_t(tile) * kN + h * S::KEYS;
+                const int key0 = tile * kN + h * S::KEYS;
                 const int slot = (v_pos(j) + h) % NSLOT;
                 ok = wait_bar(look[looks % kNotes], uint32_t(looks / kNotes) & 1u, s_abort);
                 ++looks;
@@ -950,7 +994,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 bool bad = false;
 #pragma unroll 1
                 for (int kk = lane; kk < S::KEYS; kk += 32) {
-                    const int64_t key = key0 + kk;
+                    const int key = key0 + kk;
                     if (keys_open(a, it, key, 1)) continue;  // (no row's product has a zero for it)
                     const bool seen = keys_seen(it, key, 1);
                     unsigned char* base = ring + slot * S::SLOT + (kk >> 3) * S::GROUP + (kk & 7) * 128;
@@ -983,7 +1027,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             }
         }
         if (!ok) s_abort = 1;
-    } else if (warp >= 4) {
+    } else {
         // ---- softmax: a thread a row; group w takes the tiles with j % 2 == w ----
         const int w = (warp - 4) >> 2;
         const int quarter = warp & 3;  // TMEM lanes this warp may access
@@ -996,26 +1040,38 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         int k = -1;
         float m = -INFINITY, l = 0.f;  // l: this group's share, under m
         Cut cut{0, 0, 0, -1, 0};
+        // The notes of a unit tell of the next one too, so a group reads those of its own units alone (group 1 starts
+        // with the other's first).
+        ok = wait_bar(unit_full[0], 0u, s_abort);
+        int next = ok ? s_unit[0].flags : kStop;
+        next = next & kStop ? kNextStop : ((next & kFirst ? kNextFirst : 0) | (next & kLast ? kNextLast : 0));
         for (int j = 0; ok; ++j) {
-            ok = wait_bar(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
-            const int flags = s_unit[j % kNotes].flags;
-            if (!ok || (flags & kStop)) break;
+            const bool own = (j & 1) == w;
+            int flags;
+            if (own) {
+                ok = wait_fast(unit_full[j % kNotes], uint32_t(j / kNotes) & 1u, s_abort);
+                next = flags = s_unit[j % kNotes].flags;
+                if (!ok || (flags & kStop)) break;
+            } else {
+                if (next & kNextStop) break;
+                flags = (next & kNextFirst ? kFirst : 0) | (next & kNextLast ? kLast : 0);
+            }
             if (flags & kFirst) {
                 ok = item(++k, it);
                 if (!ok) break;
                 const int rows = it.ntok * a.group;
                 valid = row < rows;
                 live = quarter * 32 < rows;  // some row of the warp is there
-                const Span v = visible(p, Request{it.tok0, it.ntok, it.len}, int64_t(it.pos0) + ti);
-                row_lo = int(v.lo);
-                row_hi = valid ? int(v.hi) : 0;
-                row_sink = valid ? int(v.sink) : 0;
+                const Keys v = keys_of(p, it.len, it.pos0 + ti);
+                row_lo = v.lo;
+                row_hi = valid ? v.hi : 0;
+                row_sink = valid ? v.sink : 0;
                 m = -INFINITY;
                 l = 0.f;
             }
             const int buf = j % NS;
-            if ((j & 1) == w) {
-                ok = wait_bar(s_full[buf], uint32_t(j / NS) & 1u, s_abort);
+            if (own) {
+                ok = wait_fast(s_full[buf], uint32_t(j / NS) & 1u, s_abort);
                 if (!ok) break;
                 tc_fence_after();
                 float mx = -INFINITY;
@@ -1040,7 +1096,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 }
                 // the running max, from the tile before (another item's is of no use, but its turn is awaited)
                 if (j > 0) {
-                    ok = wait_bar(m_ready[w ^ 1][quarter], uint32_t((j - 1) >> 1) & 1u, s_abort);
+                    ok = wait_fast(m_ready[w ^ 1][quarter], uint32_t((j - 1) >> 1) & 1u, s_abort);
                     if (!ok) break;
                 }
                 const bool first = flags & kFirst;
@@ -1116,7 +1172,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             }
             if (!ok) break;
             const uint32_t o_addr = tmem + S::O_COL + uint32_t(w * (HD / 2)) + lane_off;
-            if (s_poison[k % kNotes]) add_not_finite<HD, T>(a, it, Span{row_sink, row_lo, row_hi}, w, o_addr);
+            if (s_poison[k % kNotes]) add_not_finite<HD, T>(a, it, Keys{row_sink, row_lo, row_hi}, w, o_addr);
             const bool whole = it.u0 == 0 && it.u1 == it.units;
             if (live && whole) {
                 uint16_t* dst = static_cast<uint16_t*>(p.out) +

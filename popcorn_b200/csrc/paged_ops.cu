@@ -194,8 +194,8 @@ public:
                  v.shape_string() + ", output " + out.shape_string() + ".");
         want(R <= launch::kMaxRequests, PC_ERR_TENSOR_SHAPE_MISMATCH,
              "PagedAttention takes at most " + std::to_string(launch::kMaxRequests) + " requests; got " + std::to_string(R) + ".");
-        want(T * Nq <= kIntMax && W <= kIntMax && ps <= kIntMax && W * ps <= kIntMax && P * ps <= kIntMax,
-             PC_ERR_TENSOR_SHAPE_MISMATCH, "PagedAttention tensors are longer than int32 indices.");
+        want(T * Nq <= kIntMax && W <= kIntMax && ps <= kIntMax && W * ps <= (int64_t(1) << 30) && P * ps <= kIntMax,
+             PC_ERR_TENSOR_SHAPE_MISMATCH, "PagedAttention takes at most 2^31 - 1 query rows and slots and 2^30 keys a request.");
         ints(table, R * W, "block_table");
         ints(seq_lens, R, "seq_lens");
         ints(query_start, R + 1, "query_start");
