@@ -254,8 +254,8 @@ public:
         want(is_float(logits.dtype()), PC_ERR_UNSUPPORTED_DATA_TYPE_COMBINATION,
              "Sample logits must be f32, f16 or bf16; got " + dtype_name(logits.dtype()) + ".");
         const int64_t V = logits[logits.rank() - 1];
-        want(V >= 1 && V <= (int64_t(1) << 30), PC_ERR_TENSOR_SHAPE_MISMATCH,
-             "Sample vocabulary must be 1..2^30; got " + std::to_string(V) + ".");
+        want(V >= 1 && V <= (int64_t(1) << 21), PC_ERR_TENSOR_SHAPE_MISMATCH,  // (42-bit weights: 63-bit sums)
+             "Sample vocabulary must be 1..2^21; got " + std::to_string(V) + ".");
         const int64_t rows = logits.element_count() / V;
         want(rows <= (int64_t(1) << 27), PC_ERR_TENSOR_SHAPE_MISMATCH, "Sample takes at most 2^27 rows.");
         ints(tokens, rows, "tokens");

@@ -16,13 +16,19 @@
 //
 // One cluster of up to eight CTAs per row: the row is read from HBM once and
 // stays in the CTAs' shared memory (longer rows are read again from L2).
-// The cut of top-k / top-p is found by selection, not by sorting: a
-// histogram of counts and weights over 2048 bins linear in l_max - l (a
-// bell-shaped row spreads evenly over them, so the shared atomics rarely
-// collide), the bin where the prefix ends, and the exact order of the few
-// tokens inside it; a bin of many tokens is split again by key, and equal
-// logits are counted off by index. The draw is a two-level scan in index
-// order.
+// Nothing is sorted but a few candidates:
+//  * top-k up to 1024: the k-th largest of the threads' own maxima is not
+//    above the k-th largest logit, so a histogram of those alone (2048 bins
+//    linear in l_max - l: a bell-shaped row spreads over them and the shared
+//    atomics rarely collide) gives a border; the tokens above it, hardly more
+//    than k, go to one CTA, which orders them and does all the rest.
+//  * otherwise a histogram of all tokens' counts. A bin's weights lie within
+//    1.5 % of one another (29.9 T / 2048), so the counts and the whole weight
+//    confine the end of the top-p prefix to a few bins; a second pass sums
+//    the weights before them exactly and bins theirs. The last bin's tokens
+//    are ordered directly when they are few, split again by key when many,
+//    and counted off by index when their logits are equal.
+// The draw is a two-level scan in index order.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -40,7 +46,9 @@ using u64 = unsigned long long;
 
 constexpr int kSampleThreads = 1024;
 constexpr int kBins = 2048;
-constexpr int kCap = 256;  // tokens of a bin that are ordered directly
+constexpr int kCap = 256;     // tokens of a bin that are ordered directly
+constexpr int kList = 2048;   // candidates of a small top-k
+constexpr int kListK = 1024;  // the largest such k
 constexpr int kOneBits = 42;
 constexpr double kOne = 4398046511104.0;  // 2^42
 
@@ -51,12 +59,10 @@ struct Pick {
     int bin;                      // -1: the prefix takes everything
 };
 
-struct Shared {
+struct alignas(16) Shared {
     u64 mass[kBins], mass_all[kBins];  // (the second: sums over the cluster, in rank 0)
     uint32_t cnt[kBins], cnt_all[kBins];
-    u64 list[kCap];
-    u64 list_w[kCap];
-    double tab[32];
+    double tab[32 * 16];  // 2^(j / 32), a copy a lane of a half-warp: no bank conflicts
     u64 wsum[32], wsum2[32];
     u64 ctot[8];
     float cmax[8], cmin[8];
@@ -66,16 +72,48 @@ struct Shared {
     int32_t ia[32];
     Pick pick;
     u64 cut, cut_mass;  // the last token of the prefix, and the prefix's weight
+    int lo_bin, hi_bin;
     uint32_t list_n;
     int32_t found;
+    // (lists of candidates lie over the masses: 2048 keys, 2048 weights)
+    __device__ u64* list() { return mass; }
+    __device__ u64* list_w() { return mass_all; }
 };
+
+// NaN counts as -inf, and -0 becomes +0: equal logits have equal keys.
+__device__ __forceinline__ float tidy(float f) { return f == f ? f + 0.0f : -INFINITY; }
 
 template <class T>
 __device__ __forceinline__ float logit(const char* src, int i) {
-    float f;
-    if constexpr (Elem<T>::bytes == 4) f = reinterpret_cast<const float*>(src)[i];
-    else f = Elem<T>::load(src, i);
-    return f == f ? f + 0.0f : -INFINITY;  // (-0 becomes +0: equal logits have equal keys)
+    return tidy(Elem<T>::load(src, i));
+}
+
+// f(i, logit) for the n elements at src, 16 bytes at a time where alignment allows: thread `t` of `nt`.
+template <class T, class F>
+__device__ __forceinline__ void each(const char* src, int n, int t, int nt, F f) {
+    constexpr int es = Elem<T>::bytes, V = 16 / es;
+    int head = int((16u - (uint32_t(reinterpret_cast<uintptr_t>(src)) & 15u)) & 15u) / es;
+    head = head < n ? head : n;
+    const int nv = (n - head) / V;
+    for (int i = t; i < head; i += nt) f(i, logit<T>(src, i));
+    const uint4* v = reinterpret_cast<const uint4*>(src + head * es);
+#pragma unroll 2
+    for (int c = t; c < nv; c += nt) {
+        const uint4 x = v[c];
+        const int i = head + c * V;
+        if constexpr (es == 4) {
+            f(i, tidy(__uint_as_float(x.x)));
+            f(i + 1, tidy(__uint_as_float(x.y)));
+            f(i + 2, tidy(__uint_as_float(x.z)));
+            f(i + 3, tidy(__uint_as_float(x.w)));
+        } else {
+            float g[8];
+            unpack8<T>(x, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f(i + e, tidy(g[e]));
+        }
+    }
+    for (int i = head + nv * V + t; i < n; i += nt) f(i, logit<T>(src, i));
 }
 
 __device__ __forceinline__ uint32_t key_of(float f) {
@@ -83,28 +121,40 @@ __device__ __forceinline__ uint32_t key_of(float f) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+__device__ __forceinline__ float logit_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+// A token by its place in the order: logit first, then the earlier index; larger comes first.
+__device__ __forceinline__ u64 token_of(float l, int32_t index) {
+    return (u64(key_of(l)) << 32) | (0xffffffffu - uint32_t(index));
+}
+
 struct Weight {
     float lmax, live;  // live: l_max - l above it weighs zero
-    double c;          // log2(e) / T
-    const double* tab;
+    double top, c32;   // l_max; 32 log2(e) / T
+    const double* tab;  // this lane's copy
 
     __device__ __forceinline__ bool is_live(float l) const {
         return l == lmax || (l > -INFINITY && lmax - l <= live);
     }
+    // 2^42 exp((l - l_max) / T) to the nearest integer. With k = 32 log2 of the exponential and n the integer next to
+    // it: 2^(n / 32), from a table and an exponent, times 2^((k - n) / 32), |k - n| <= 1/2, by its series to the fifth
+    // power (the sixth is below 2^-48). Adding 1.5 2^52 or 2^52 leaves the nearest integer in a double's low bits.
     __device__ __forceinline__ u64 operator()(float l) const {
         if (l == lmax) return u64(1) << kOneBits;
-        if (!(lmax - l <= live)) return 0;
-        const double t = (double(l) - double(lmax)) * c;
-        if (!(t >= -43.0)) return 0;
-        const int n = __double2int_rn(t * 32.0);
-        const double x = fma(double(n), -1.0 / 32.0, t) * 0.6931471805599453;  // |x| <= ln 2 / 64
-        double e = fma(x, 1.0 / 120.0, 1.0 / 24.0);
-        e = fma(e, x, 1.0 / 6.0);
-        e = fma(e, x, 0.5);
+        const double k = (double(l) - top) * c32;
+        if (!(lmax - l <= live) || !(k >= -43.0 * 32.0)) return 0;
+        const double r = k + 6755399441055744.0;
+        const int n = __double2loint(r);
+        const double x = k - (r - 6755399441055744.0);
+        double e = fma(x, 3.9737099845494154e-11, 9.172562701824643e-09);  // (ln 2 / 32)^i / i!
+        e = fma(e, x, 1.6938509724371819e-06);
+        e = fma(e, x, 2.3459619820224677e-04);
+        e = fma(e, x, 2.166084939249829e-02);
         e = fma(e, x, 1.0);
-        e = fma(e, x, 1.0);
-        const double scale = __longlong_as_double((long long)(1023 + kOneBits + (n >> 5)) << 52);
-        return __double2ull_rn(tab[n & 31] * e * scale);
+        const double t = tab[(n & 31) * 16];
+        const double s = __hiloint2double(__double2hiint(t) + ((kOneBits + (n >> 5)) << 20), __double2loint(t));
+        return u64(__double_as_longlong(fma(e, s, 4503599627370496.0))) & ((u64(1) << 52) - 1);
     }
 };
 
@@ -135,18 +185,22 @@ struct Cluster {
     }
 };
 
+// The tokens [s0, s1) of a CTA's (or of a part of them) that belong to a warp.
+__device__ __forceinline__ void segment(int n, int warp, int& s0, int& s1) {
+    const int seg = ((n + 31) / 32 + 31) / 32 * 32;
+    s0 = warp * seg < n ? warp * seg : n;
+    s1 = s0 + seg < n ? s0 + seg : n;
+}
+
 // First index (in index order, over the cluster) whose running sum of
-// value(i) exceeds target(total); every thread of the cluster calls it and
-// learns the index (-1: none).
-template <class V, class G>
-__device__ int32_t locate(const Cluster& cl, int n, int32_t base, V value, G target) {
+// value(i, logit) exceeds target(total), given `acc`, the sum over this warp's
+// segment; every thread of the cluster calls it and learns the index (-1:
+// none). The CTA that holds it looks at one warp's segment with all of its
+// warps, and one of these at a 32nd of that.
+template <class T, class V, class G>
+__device__ int32_t find(const Cluster& cl, const char* src, int n, int32_t base, u64 acc, V value, G target) {
     Shared* sh = cl.sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int seg = ((n + 31) / 32 + 31) / 32 * 32;
-    const int s0 = warp * seg, s1 = s0 + seg < n ? s0 + seg : n;
-    u64 acc = 0;
-    for (int i = s0 + lane; i < s1; i += 32) acc += value(i);
-    acc = warp_sum64(acc);
     if (lane == 0) sh->wsum[warp] = acc;
     if (tid == 0) sh->found = -1;
     __syncthreads();
@@ -155,24 +209,45 @@ __device__ int32_t locate(const Cluster& cl, int n, int32_t base, V value, G tar
         if (lane < cl.C) cl.of(lane)->ctot[cl.rank] = mine;
     }
     cl.sync();
-    u64 total = 0, run = 0;
+    u64 total = 0, run = 0, mine = 0;
     for (int r = 0; r < cl.C; ++r) {
-        if (r == cl.rank) run = total;
+        if (r == cl.rank) {
+            run = total;
+            mine = sh->ctot[r];
+        }
         total += sh->ctot[r];
     }
     const double goal = target(total);
-    for (int w = 0; w < warp; ++w) run += sh->wsum[w];
-    if (acc > 0 && double(run) <= goal && goal < double(run + acc)) {  // this warp's segment holds it
-        for (int i0 = s0; i0 < s1; i0 += 32) {
-            const u64 v = i0 + lane < s1 ? value(i0 + lane) : 0;
-            const u64 incl = warp_scan64(v, lane);
-            const unsigned hit = __ballot_sync(0xffffffffu, double(run + incl) > goal);
-            if (hit) {
-                const int32_t at = base + i0 + (__ffs(int(hit)) - 1);
-                if (lane < cl.C) cl.of(lane)->found = at;
-                break;
+    if (mine > 0 && double(run) <= goal && goal < double(run + mine)) {  // (the same for the whole CTA)
+        // the warp's segment that holds it
+        const u64 in1 = run + warp_scan64(sh->wsum[lane], lane);
+        const int w1 = __ffs(int(__ballot_sync(0xffffffffu, double(in1) > goal))) - 1;
+        run = w1 > 0 ? __shfl_sync(0xffffffffu, in1, (w1 - 1) & 31) : run;
+        int b0, b1, s0, s1;
+        segment(n, w1 < 0 ? 31 : w1, b0, b1);
+        segment(b1 - b0, warp, s0, s1);
+        s0 += b0;
+        s1 += b0;
+        u64 part = 0;
+        for (int i = s0 + lane; i < s1; i += 32) part += value(i, logit<T>(src, i));
+        part = warp_sum64(part);
+        if (lane == 0) sh->wsum2[warp] = part;
+        __syncthreads();
+        const u64 in2 = run + warp_scan64(sh->wsum2[lane], lane);
+        const int w2 = __ffs(int(__ballot_sync(0xffffffffu, double(in2) > goal))) - 1;
+        run = warp > 0 ? __shfl_sync(0xffffffffu, in2, (warp - 1) & 31) : run;
+        if (warp == w2) {
+            for (int i0 = s0; i0 < s1; i0 += 32) {
+                const u64 v = i0 + lane < s1 ? value(i0 + lane, logit<T>(src, i0 + lane)) : 0;
+                const u64 incl = warp_scan64(v, lane);
+                const unsigned hit = __ballot_sync(0xffffffffu, double(run + incl) > goal);
+                if (hit) {
+                    const int32_t at = base + i0 + (__ffs(int(hit)) - 1);
+                    if (lane < cl.C) cl.of(lane)->found = at;
+                    break;
+                }
+                run += __shfl_sync(0xffffffffu, incl, 31);
             }
-            run += __shfl_sync(0xffffffffu, incl, 31);
         }
     }
     cl.sync();
@@ -181,36 +256,57 @@ __device__ int32_t locate(const Cluster& cl, int n, int32_t base, V value, G tar
     return at;
 }
 
-// Histogram of the tokens that bin(l) >= 0 places, summed over the cluster
-// into rank 0, and the bin in which the prefix of `goal` ends: by count
-// (by_mass false: the goal-th token) or by weight (the first token with
-// which the weight reaches goal), `before` of either already above it.
-template <class T, class B>
-__device__ void histogram(const Cluster& cl, const char* src, int n, const Weight& w, bool masses, B bin) {
+template <class T, class V, class G>
+__device__ int32_t locate(const Cluster& cl, const char* src, int n, int32_t base, V value, G target) {
+    int s0, s1;
+    segment(n, threadIdx.x >> 5, s0, s1);
+    u64 acc = 0;
+    each<T>(src + int64_t(s0) * Elem<T>::bytes, s1 - s0, threadIdx.x & 31, 32, [&](int i, float l) { acc += value(s0 + i, l); });
+    return find<T>(cl, src, n, base, warp_sum64(acc), value, target);
+}
+
+// The sum over the cluster's threads.
+__device__ u64 cluster_sum(const Cluster& cl, u64 acc) {
     Shared* sh = cl.sh;
-    const int tid = threadIdx.x;
-    for (int b = tid; b < kBins; b += kSampleThreads) {
-        sh->cnt[b] = 0;
-        sh->mass[b] = 0;
-    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    acc = warp_sum64(acc);
+    if (lane == 0) sh->wsum[warp] = acc;
     __syncthreads();
-    for (int i = tid; i < n; i += kSampleThreads) {
-        const float l = logit<T>(src, i);
-        const int b = bin(l);
-        if (b >= 0) {
-            atomicAdd(&sh->cnt[b], 1u);
-            if (masses) {
-                const u64 v = w(l);
-                if (v) atomicAdd(&sh->mass[b], v);
-            }
-        }
+    if (warp == 0) {
+        const u64 mine = warp_sum64(sh->wsum[lane]);
+        if (lane < cl.C) cl.of(lane)->ctot[cl.rank] = mine;
     }
     cl.sync();
+    u64 total = 0;
+    for (int r = 0; r < cl.C; ++r) total += sh->ctot[r];
+    cl.sync();
+    return total;
+}
+
+// value summed over the cluster's tokens, exactly.
+template <class T, class V>
+__device__ u64 total_of(const Cluster& cl, const char* src, int n, V value) {
+    u64 acc = 0;
+    each<T>(src, n, threadIdx.x, kSampleThreads, [&](int, float l) { acc += value(l); });
+    return cluster_sum(cl, acc);
+}
+
+__device__ void clear_bins(const Cluster& cl, bool masses) {
+    for (int b = threadIdx.x; b < kBins; b += kSampleThreads) {
+        cl.sh->cnt[b] = 0;
+        if (masses) cl.sh->mass[b] = 0;
+    }
+    __syncthreads();
+}
+
+// The cluster's bins summed into rank 0.
+__device__ void gather_bins(const Cluster& cl, bool masses) {
+    cl.sync();
     Shared* lead = cl.of(0);
-    const int per = kBins / cl.C;
-    for (int b = cl.rank * per + tid; b < (cl.rank + 1) * per; b += kSampleThreads) {
+    for (int b = cl.rank + cl.C * int(threadIdx.x); b < kBins; b += cl.C * kSampleThreads) {
         u64 m = 0;
         uint32_t c = 0;
+#pragma unroll 4
         for (int r = 0; r < cl.C; ++r) {
             const Shared* o = cl.of(r);
             c += o->cnt[b];
@@ -222,6 +318,25 @@ __device__ void histogram(const Cluster& cl, const char* src, int n, const Weigh
     cl.sync();
 }
 
+// Histogram of the tokens that bin(l) >= 0 places (their weights too), summed over the cluster into rank 0.
+template <class T, class B>
+__device__ void histogram(const Cluster& cl, const char* src, int n, const Weight& w, bool masses, B bin) {
+    Shared* sh = cl.sh;
+    clear_bins(cl, masses);
+    each<T>(src, n, threadIdx.x, kSampleThreads, [&](int, float l) {
+        const int b = bin(l);
+        if (b < 0) return;
+        atomicAdd(&sh->cnt[b], 1u);
+        if (masses) {
+            const u64 v = w(l);
+            if (v) atomicAdd(&sh->mass[b], v);
+        }
+    });
+    gather_bins(cl, masses);
+}
+
+// The bin in which the prefix of `goal` ends: by count (the goal-th token) or by weight (the first token with which the
+// weight reaches goal), `before` of either already above it.
 __device__ Pick pick_bin(const Cluster& cl, bool by_mass, double goal, u64 before_cnt, u64 before_mass) {
     Shared* sh = cl.sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -261,89 +376,86 @@ __device__ Pick pick_bin(const Cluster& cl, bool by_mass, double goal, u64 befor
     return p;
 }
 
-// The prefix's last token inside the picked bin; sets sh->cut (a token's key
-// and index, larger = earlier) and sh->cut_mass (the prefix's weight).
-template <class T>
-__device__ void resolve(const Cluster& cl, const char* src, int n, int32_t base, const Weight& w, float scale,
-                        bool by_mass, double goal, bool masses, Pick p) {
+// The prefix's last token among the p.n listed ones of its bin; sets sh->cut (a token's key and index, larger =
+// earlier) and sh->cut_mass (the prefix's weight).
+__device__ void order_list(const Cluster& cl, const Weight& w, bool by_mass, double goal, bool masses, const Pick& p) {
+    Shared* sh = cl.sh;
+    const int tid = threadIdx.x;
+    cl.sync();
+    if (cl.rank == 0) {
+        const int cnt = int(p.n);
+        u64 me = 0, wm = 0, above = 0;
+        int place = 0;
+        if (tid < cnt) {
+            me = sh->list()[tid];
+            wm = masses ? w(logit_of(uint32_t(me >> 32))) : 0;
+            sh->list_w()[tid] = wm;
+        }
+        __syncthreads();
+        if (tid < cnt) {
+            for (int j = 0; j < cnt; ++j)
+                if (sh->list()[j] > me) {
+                    ++place;
+                    above += sh->list_w()[j];
+                }
+            const u64 ec = p.before_cnt + u64(place), em = p.before_mass + above;
+            const bool last =
+                by_mass ? double(em) < goal && goal <= double(em + wm) : double(ec) < goal && goal <= double(ec + 1);
+            if (last) {
+                sh->cut = me;
+                sh->cut_mass = em + wm;
+            }
+        }
+        __syncthreads();
+        const u64 cut = sh->cut, mass = sh->cut_mass;
+        if (tid < cl.C && tid > 0) {
+            Shared* o = cl.of(tid);
+            o->cut = cut;
+            o->cut_mass = mass;
+        }
+    }
+    cl.sync();
+}
+
+// As order_list, from the tokens that in_bin(logit) tells.
+template <class T, class B>
+__device__ void resolve(const Cluster& cl, const char* src, int n, int32_t base, const Weight& w, bool by_mass, double goal,
+                        bool masses, Pick p, B in_bin) {
     Shared* sh = cl.sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // members: the d-bin `p.bin` first, then a range of keys
+    // members: the picked bin first, then a range of keys
     bool by_key = false;
     uint32_t klo = 0, khi = 0;
-    const int dbin = p.bin;
-    auto d_bin = [&](float l) {
-        if (!w.is_live(l)) return -1;
-        const float d = l == w.lmax ? 0.f : w.lmax - l;
-        const int b = int(d * scale);
-        return b < 0 ? 0 : (b >= kBins ? kBins - 1 : b);
-    };
     auto member = [&](float l) {
         if (by_key) {
             const uint32_t k = key_of(l);
             return k >= klo && k <= khi;
         }
-        return d_bin(l) == dbin;
+        return bool(in_bin(l));
     };
     for (;;) {
         if (p.n <= kCap) {
             if (tid == 0) sh->list_n = 0;
             cl.sync();
             Shared* lead = cl.of(0);
-            for (int i = tid; i < n; i += kSampleThreads) {
-                const float l = logit<T>(src, i);
+            each<T>(src, n, tid, kSampleThreads, [&](int i, float l) {
                 if (member(l)) {
                     const uint32_t at = atomicAdd(&lead->list_n, 1u);
-                    if (at < kCap) lead->list[at] = (u64(key_of(l)) << 32) | (0xffffffffu - uint32_t(base + i));
+                    if (at < kCap) lead->list()[at] = token_of(l, base + i);
                 }
-            }
-            cl.sync();
-            if (cl.rank == 0) {
-                const int cnt = int(p.n);
-                u64 me = 0, wm = 0, above = 0;
-                int place = 0;
-                if (tid < cnt) {
-                    me = sh->list[tid];
-                    const uint32_t k = uint32_t(me >> 32);
-                    wm = masses ? w(__uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k)) : 0;
-                    sh->list_w[tid] = wm;
-                }
-                __syncthreads();
-                if (tid < cnt) {
-                    for (int j = 0; j < cnt; ++j)
-                        if (sh->list[j] > me) {
-                            ++place;
-                            above += sh->list_w[j];
-                        }
-                    const u64 ec = p.before_cnt + u64(place), em = p.before_mass + above;
-                    const bool last = by_mass ? double(em) < goal && goal <= double(em + wm)
-                                              : double(ec) < goal && goal <= double(ec + 1);
-                    if (last) {
-                        sh->cut = me;
-                        sh->cut_mass = em + wm;
-                    }
-                }
-                __syncthreads();
-                const u64 cut = sh->cut, mass = sh->cut_mass;
-                if (tid < cl.C && tid > 0) {
-                    Shared* o = cl.of(tid);
-                    o->cut = cut;
-                    o->cut_mass = mass;
-                }
-            }
-            cl.sync();
+            });
+            order_list(cl, w, by_mass, goal, masses, p);
             return;
         }
         // the members' smallest and largest keys
         uint32_t kmin = 0xffffffffu, kmax = 0;
-        for (int i = tid; i < n; i += kSampleThreads) {
-            const float l = logit<T>(src, i);
+        each<T>(src, n, tid, kSampleThreads, [&](int, float l) {
             if (member(l)) {
                 const uint32_t k = key_of(l);
                 kmin = k < kmin ? k : kmin;
                 kmax = k > kmax ? k : kmax;
             }
-        }
+        });
         kmin = __reduce_min_sync(0xffffffffu, kmin);
         kmax = __reduce_max_sync(0xffffffffu, kmax);
         if (lane == 0) {
@@ -369,7 +481,7 @@ __device__ void resolve(const Cluster& cl, const char* src, int n, int32_t base,
         }
         if (kmin == kmax) {
             // equal logits: the q-th of them in index order ends the prefix
-            const u64 wk = masses ? w(__uint_as_float(kmin & 0x80000000u ? kmin & 0x7fffffffu : ~kmin)) : 0;
+            const u64 wk = masses ? w(logit_of(kmin)) : 0;
             u64 q;
             if (by_mass) {
                 q = wk ? u64((goal - double(p.before_mass)) / double(wk)) : 1;
@@ -379,8 +491,8 @@ __device__ void resolve(const Cluster& cl, const char* src, int n, int32_t base,
                 q = u64(goal) - p.before_cnt;
             }
             q = q < 1 ? 1 : (q > p.n ? p.n : q);
-            const int32_t at = locate(
-                cl, n, base, [&](int i) { return u64(key_of(logit<T>(src, i)) == kmin ? 1 : 0); },
+            const int32_t at = locate<T>(
+                cl, src, n, base, [&](int, float l) { return u64(key_of(l) == kmin ? 1 : 0); },
                 [&](u64) { return double(q - 1); });
             if (tid == 0) {
                 sh->cut = (u64(kmin) << 32) | (0xffffffffu - uint32_t(at));
@@ -407,36 +519,221 @@ __device__ void resolve(const Cluster& cl, const char* src, int n, int32_t base,
     }
 }
 
+// Descending bitonic sort of m (a power of two, 64 .. kList) keys, two neighbours a thread: pairs up to 32 apart are a
+// thread's own or change lanes by shuffles, the others go through shared memory.
+__device__ void sort_down(u64* a, int m) {
+    const int tid = threadIdx.x;
+    const bool on = 2 * tid < m;  // (whole warps)
+    u64 v0 = 0, v1 = 0;
+    __syncthreads();
+    if (on) {
+        v0 = a[2 * tid];
+        v1 = a[2 * tid + 1];
+    }
+#pragma unroll 1
+    for (int k = 2; k <= m; k <<= 1) {
+        const bool down = (2 * tid & k) == 0;
+#pragma unroll 1
+        for (int j = k >> 1; j >= 64; j >>= 1) {
+            __syncthreads();
+            if (on) {
+                a[2 * tid] = v0;
+                a[2 * tid + 1] = v1;
+            }
+            __syncthreads();
+            if (on) {
+                const u64 o0 = a[(2 * tid) ^ j], o1 = a[(2 * tid + 1) ^ j];
+                const bool large = ((2 * tid & j) == 0) == down;  // this one keeps the larger
+                v0 = (v0 < o0) == large ? o0 : v0;
+                v1 = (v1 < o1) == large ? o1 : v1;
+            }
+        }
+        if (on) {
+#pragma unroll 1
+            for (int j = k >> 1 < 32 ? k >> 1 : 32; j >= 2; j >>= 1) {
+                const u64 o0 = __shfl_xor_sync(0xffffffffu, v0, j >> 1), o1 = __shfl_xor_sync(0xffffffffu, v1, j >> 1);
+                const bool large = ((2 * tid & j) == 0) == down;
+                v0 = (v0 < o0) == large ? o0 : v0;
+                v1 = (v1 < o1) == large ? o1 : v1;
+            }
+            if ((v0 < v1) == down) {
+                const u64 t = v0;
+                v0 = v1;
+                v1 = t;
+            }
+        }
+    }
+    __syncthreads();
+    if (on) {
+        a[2 * tid] = v0;
+        a[2 * tid + 1] = v1;
+    }
+    __syncthreads();
+}
+
+// Inclusive sums of v over the CTA's threads, and the total.
+__device__ u64 scan_cta(u64 v, u64& total, u64* wsum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 incl = warp_scan64(v, lane);
+    __syncthreads();
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    if (warp == 0) wsum[lane] = warp_scan64(wsum[lane], lane);
+    __syncthreads();
+    total = wsum[31];
+    return incl + (warp ? wsum[warp - 1] : 0);
+}
+
+// The bins sh->lo_bin .. hi_bin in which the prefix of weight `goal` may end, from the counts alone: a bin's tokens weigh
+// between its borders' weights, half a unit each way for the weights' own rounding. (2^-16 of slack: of an exponent of at
+// most 29.9, l_max - l, the scale, their product and the border's exponent are each off by 2^-24 of it, exp2f by a little.)
+__device__ void end_bins(const Cluster& cl, double temp, float scale, double goal) {
+    Shared* sh = cl.sh;
+    const int tid = threadIdx.x;
+    if (cl.rank == 0) {
+        const double step = scale > 0.f ? 1.4426950408889634 / (temp * double(scale)) : 0.0;  // log2 a bin
+        u64 hi[2], lo[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int b = 2 * tid + e;
+            const double c = double(sh->cnt_all[b]);
+            hi[e] = u64(c * (kOne * double(exp2f(float(-step * b))) * (1.0 + 0x1p-16) + 0.5)) + 1;
+            lo[e] = scale > 0.f ? u64(c * fmax(kOne * double(exp2f(float(-step * (b + 1)))) * (1.0 - 0x1p-16) - 0.5, 0.0)) : 0;
+        }
+        if (tid == 0) sh->lo_bin = sh->hi_bin = kBins - 1;
+        u64 total;
+        const u64 th = scan_cta(hi[0] + hi[1], total, sh->wsum), tl = scan_cta(lo[0] + lo[1], total, sh->wsum2);
+        // the first bin with which the sum from above reaches the goal, and that from below
+        if (double(th) >= goal) atomicMin(&sh->lo_bin, double(th - hi[1]) >= goal ? 2 * tid : 2 * tid + 1);
+        if (double(tl) >= goal) atomicMin(&sh->hi_bin, double(tl - lo[1]) >= goal ? 2 * tid : 2 * tid + 1);
+        __syncthreads();
+        const int a = sh->lo_bin, b = sh->hi_bin;
+        if (tid < cl.C && tid > 0) {
+            cl.of(tid)->lo_bin = a;
+            cl.of(tid)->hi_bin = b;
+        }
+    }
+    cl.sync();
+}
+
+// The token from a list of candidates (keys and indices) that holds the k first ones; one CTA.
+__device__ int32_t draw_from_list(Shared* sh, int n, int k, const Weight& w, float top_p, double min_w, float u) {
+    const int tid = threadIdx.x;
+    u64* list = sh->list();
+    u64* lw = sh->list_w();
+    int m = 64;
+    while (m < n) m <<= 1;
+    for (int i = n + tid; i < m; i += kSampleThreads) list[i] = 0;
+    sort_down(list, m);
+    n = n < k ? n : k;
+    // two neighbours a thread
+    u64 v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        const uint32_t key = i < n ? uint32_t(list[i] >> 32) : 0;
+        v[e] = i < n ? w(logit_of(key)) : 0;
+    }
+    u64 total;
+    const u64 incl = scan_cta(v[0] + v[1], total, sh->wsum);
+    const double goal = top_p < 1.f ? fmax(double(top_p) * double(total), 1.0) : 1e300;
+    // kept: before it the weight has not reached the goal, and it weighs enough; then in index order
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        const u64 before = incl - v[1] - (e ? 0 : v[0]);
+        const bool keep = i < n && double(before) < goal && double(v[e]) >= min_w && v[e] > 0;
+        // (the list's low words hold 2^32 - 1 - index: a larger one is an earlier token)
+        const u64 id = keep ? (list[i] << 32) | uint32_t(i) : 0;
+        lw[i] = keep ? v[e] : 0;
+        v[e] = id;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (2 * tid + e < m) list[2 * tid + e] = v[e];
+    sort_down(list, m);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        v[e] = i < m && list[i] ? lw[uint32_t(list[i])] : 0;
+    }
+    u64 kept;
+    const u64 sum = scan_cta(v[0] + v[1], kept, sh->wsum);
+    const double at = double(u) * double(kept);
+    if (tid == 0) sh->found = -1;
+    __syncthreads();
+    const u64 b0 = sum - v[0] - v[1], b1 = sum - v[1];
+    if (v[0] && double(b0) <= at && at < double(b1)) sh->found = int32_t(0xffffffffu - uint32_t(list[2 * tid] >> 32));
+    if (v[1] && double(b1) <= at && at < double(sum)) sh->found = int32_t(0xffffffffu - uint32_t(list[2 * tid + 1] >> 32));
+    __syncthreads();
+    return sh->found;
+}
+
 template <class T>
 __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample p, int C, int chunk, int resident) {
     extern __shared__ __align__(16) char smem[];
     Shared* sh = reinterpret_cast<Shared*>(smem);
-    char* data = smem + sizeof(Shared);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Cluster cl{sh, C, int(blockIdx.x % unsigned(C))};
     const int64_t row = blockIdx.x / unsigned(C);
-    if (tid < 32) sh->tab[tid] = exp2(double(tid) / 32.0);
+    if (tid < 512) sh->tab[tid] = exp2(double(tid >> 4) / 32.0);
+    if (C > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // (this CTA runs)
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int es = Elem<T>::bytes;
+    constexpr int es = Elem<T>::bytes, V = 16 / es;
     const int32_t base = cl.rank * chunk;
     const int n = p.V - base < chunk ? (p.V > base ? int(p.V - base) : 0) : chunk;
     const char* global = static_cast<const char*>(p.logits) + (row * p.V + base) * es;
+    // (in shared memory at the same distance from a 16-byte border)
+    char* data = smem + sizeof(Shared) + (reinterpret_cast<uintptr_t>(global) & 15u);
     const char* src = resident ? data : global;
 
     // the row's largest (and, for the histogram's range, smallest) logit
     float mx = -INFINITY, mn = INFINITY;
     int32_t mi = 0x7fffffff;
-    for (int i = tid; i < n; i += kSampleThreads) {
-        using S = typename T::storage;
-        if (resident) reinterpret_cast<S*>(data)[i] = reinterpret_cast<const S*>(global)[i];
-        const float l = logit<T>(global, i);
+    auto look = [&](int i, float l) {
         if (l > mx) {
             mx = l;
             mi = base + i;
         }
         if (l > -INFINITY) mn = fminf(mn, l);
+    };
+    if (resident) {
+        int head = int((16u - (uint32_t(reinterpret_cast<uintptr_t>(global)) & 15u)) & 15u) / es;
+        head = head < n ? head : n;
+        const int nv = (n - head) / V;
+        using S = typename T::storage;
+        auto one = [&](int i) {
+            reinterpret_cast<S*>(data)[i] = reinterpret_cast<const S*>(global)[i];
+            look(i, logit<T>(global, i));
+        };
+        if (tid < head) one(tid);
+        const uint4* g = reinterpret_cast<const uint4*>(global + head * es);
+        uint4* d = reinterpret_cast<uint4*>(data + head * es);
+#pragma unroll 4
+        for (int c = tid; c < nv; c += kSampleThreads) {
+            const uint4 x = g[c];
+            d[c] = x;
+            const int i = head + c * V;
+            if constexpr (es == 4) {
+                look(i, tidy(__uint_as_float(x.x)));
+                look(i + 1, tidy(__uint_as_float(x.y)));
+                look(i + 2, tidy(__uint_as_float(x.z)));
+                look(i + 3, tidy(__uint_as_float(x.w)));
+            } else {
+                float f[8];
+                unpack8<T>(x, f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) look(i + e, tidy(f[e]));
+            }
+        }
+        if (tid < n - head - nv * V) one(head + nv * V + tid);
+    } else {
+        each<T>(global, n, tid, kSampleThreads, look);
     }
+    const float own = mx;  // this thread's largest
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float om = __shfl_xor_sync(0xffffffffu, mx, o);
@@ -453,6 +750,8 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         sh->ia[warp] = mi;
     }
     __syncthreads();
+    // every CTA of the cluster is running before its memory is written
+    if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (warp == 0) {
         mx = sh->fa[lane];
         mn = sh->fb[lane];
@@ -467,16 +766,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
             }
             mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
         }
-        // every CTA of the cluster is running before its memory is written
-        if (C > 1) cg::this_cluster().sync();
         if (lane < C) {
             Shared* o = cl.of(lane);
             o->cmax[cl.rank] = mx;
             o->cmin[cl.rank] = mn;
             o->cidx[cl.rank] = mi;
         }
-    } else if (C > 1) {
-        cg::this_cluster().sync();
     }
     cl.sync();
     mx = -INFINITY;
@@ -494,74 +789,193 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         if (cl.rank == 0 && tid == 0) p.tokens[row] = mx == -INFINITY ? -1 : mi;
         return;  // no CTA touches another's memory after the barrier above
     }
-    Weight w{mx, 29.9f * temp, 1.4426950408889634 / double(temp), sh->tab};
+    const Weight w{mx, 29.9f * temp, double(mx), 32.0 * 1.4426950408889634 / double(temp), sh->tab + (lane & 15)};
     const int32_t k = p.top_k ? p.top_k[row] : 0;
     const float tp = p.top_p ? p.top_p[row] : 1.f;
-    float mp = p.min_p ? p.min_p[row] : 0.f;
+    const float mp = p.min_p ? p.min_p[row] : 0.f;
     const double min_w = mp > 0.f ? double(fminf(mp, 1.f)) * kOne : 0.0;
+    const float u = fminf(fmaxf(p.uniform[row], 0.f), 0.99999994f);
     const bool use_k = k > 0 && k < p.V, use_p = tp < 1.f;  // (NaN: off)
     u64 cut = 0;  // every token
+    u64 acc = 0;  // the kept weight of this warp's segment
+    bool summed = false;
     if (use_k || use_p) {
         const float range = fminf(mx - mn, w.live);
-        const float scale = range > 0.f ? float(kBins) / range : 0.f;
+        const float scale = range > 0.f ? fminf(float(kBins) / range, 1e30f) : 0.f;
         auto d_bin = [&](float l) {
             if (!w.is_live(l)) return -1;
             const float d = l == mx ? 0.f : mx - l;
             const int b = int(d * scale);
             return b < 0 ? 0 : (b >= kBins ? kBins - 1 : b);
         };
-        histogram<T>(cl, src, n, w, use_p, d_bin);
+        if (use_k && k <= kListK) {
+            // the border: from the threads' maxima, or from all tokens where those are too few to tell
+            const bool by_max = k <= kSampleThreads * C / 4;
+            Pick b;
+            if (by_max) {
+                clear_bins(cl, false);
+                const int at = d_bin(own);
+                if (at >= 0) atomicAdd(&sh->cnt[at], 1u);
+                gather_bins(cl, false);
+                b = pick_bin(cl, false, double(k), 0, 0);
+            }
+            if (!by_max || b.bin < 0) {
+                histogram<T>(cl, src, n, w, false, d_bin);
+                b = pick_bin(cl, false, double(k), 0, 0);
+            }
+            const int border = b.bin < 0 ? kBins - 1 : b.bin;
+            if (tid == 0) sh->list_n = 0;
+            cl.sync();
+            Shared* lead = cl.of(0);
+            const float end = border < kBins - 1 ? float(border + 1) : INFINITY;
+            each<T>(src, n, tid, kSampleThreads, [&](int i, float l) {
+                if (!((mx - l) * scale >= end) && w.is_live(l)) {  // (NaN: infinite logits)
+                    const uint32_t to = atomicAdd(&lead->list_n, 1u);
+                    if (to < kList) lead->list()[to] = token_of(l, base + i);
+                }
+            });
+            cl.sync();
+            const uint32_t found = lead->list_n;
+            cl.sync();  // (the last look at another CTA's memory, if the list is complete)
+            if (found <= kList) {
+                if (cl.rank == 0) {
+                    const int32_t token = draw_from_list(sh, int(found), k, w, tp, min_w, u);
+                    if (tid == 0) p.tokens[row] = token;
+                }
+                return;
+            }
+        }
+        // by the counts of all tokens
         double mass = 0.0;
+        bool whole = true;  // top-k takes every token that weighs
         if (use_k) {
-            const Pick pk = pick_bin(cl, false, double(k), 0, 0);
-            mass = double(pk.total_mass);
+            histogram<T>(cl, src, n, w, false, d_bin);
+            Pick pk = pick_bin(cl, false, double(k), 0, 0);
             if (pk.bin >= 0) {
-                resolve<T>(cl, src, n, base, w, scale, false, double(k), use_p, pk);
+                whole = false;
+                if (use_p) {
+                    pk.before_mass = total_of<T>(cl, src, n, [&](float l) {
+                        const int b = d_bin(l);
+                        return b >= 0 && b < pk.bin ? w(l) : u64(0);
+                    });
+                }
+                resolve<T>(cl, src, n, base, w, false, double(k), use_p, pk, [&](float l) { return d_bin(l) == pk.bin; });
                 cut = sh->cut;
                 mass = double(sh->cut_mass);
-                if (use_p && pk.n > kCap) histogram<T>(cl, src, n, w, true, d_bin);  // (resolve wrote over it)
             }
         }
         if (use_p) {
-            if (!use_k) {
-                // the whole weight: a goal beyond it picks nothing
-                mass = double(pick_bin(cl, true, 1e300, 0, 0).total_mass);
-            }
+            clear_bins(cl, false);
+            const u64 all = total_of<T>(cl, src, n, [&](float l) -> u64 {
+                const int b = d_bin(l);
+                if (b < 0) return 0;
+                atomicAdd(&sh->cnt[b], 1u);
+                return whole ? w(l) : 0;
+            });
+            gather_bins(cl, false);
+            if (whole) mass = double(all);
             const double goal = fmax(double(tp) * mass, 1.0);  // (p <= 0: the first token alone)
-            const Pick pp = pick_bin(cl, true, goal, 0, 0);
-            if (pp.bin >= 0) {
-                resolve<T>(cl, src, n, base, w, scale, true, goal, true, pp);
+            end_bins(cl, double(temp), scale, goal);
+            const int b0 = sh->lo_bin, b1 = sh->hi_bin;
+            // the weight before them exactly, and theirs by a 2048th of them; a warp's segment at a time, since the
+            // draw wants the kept weight of each
+            const float first = float(b0), fine = float(kBins) / float(b1 + 1 - b0);
+            auto f_bin = [&](float l) {  // of a token in b0 .. b1: rises with l_max - l
+                const float f = l == mx ? 0.f : (mx - l) * scale;
+                const int b = int((f - first) * fine);
+                return b < 0 ? 0 : (b >= kBins ? kBins - 1 : b);
+            };
+            int s0, s1;
+            segment(n, warp, s0, s1);
+            const char* part = src + int64_t(s0) * es;
+            clear_bins(cl, true);
+            u64 before = 0, kept = 0;
+            each<T>(part, s1 - s0, lane, 32, [&](int, float l) {
+                const int b = d_bin(l);
+                if (b < 0 || b > b1) return;
+                const u64 v = w(l);
+                if (b < b0) {
+                    before += v;
+                    if (double(v) >= min_w) kept += v;
+                    return;
+                }
+                const int f = f_bin(l);
+                atomicAdd(&sh->cnt[f], 1u);
+                if (v) atomicAdd(&sh->mass[f], v);
+            });
+            before = cluster_sum(cl, before);
+            gather_bins(cl, true);
+            const Pick pp = pick_bin(cl, true, goal, 0, before);
+            if (pp.bin >= 0 && pp.n <= kCap) {
+                // list the bin's tokens, and add to each segment's kept weight those before them
+                if (tid == 0) sh->list_n = 0;
+                cl.sync();
+                Shared* lead = cl.of(0);
+                each<T>(part, s1 - s0, lane, 32, [&](int i, float l) {
+                    const int b = d_bin(l);
+                    if (b < b0 || b > b1) return;
+                    const int f = f_bin(l);
+                    if (f < pp.bin) {
+                        const u64 v = w(l);
+                        if (double(v) >= min_w) kept += v;
+                    } else if (f == pp.bin) {
+                        const uint32_t at = atomicAdd(&lead->list_n, 1u);
+                        if (at < kCap) lead->list()[at] = token_of(l, base + s0 + i);
+                    }
+                });
+                order_list(cl, w, true, goal, true, pp);
+                cut = sh->cut;
+                // and of the listed ones those that are in the prefix
+                for (int j = lane; j < int(pp.n); j += 32) {
+                    const u64 t = lead->list()[j];
+                    const int32_t at = int32_t(0xffffffffu - uint32_t(t)) - base;
+                    if (t >= cut && at >= s0 && at < s1) {
+                        const u64 v = w(logit_of(uint32_t(t >> 32)));
+                        if (double(v) >= min_w) kept += v;
+                    }
+                }
+                summed = true;
+                acc = warp_sum64(kept);
+            } else if (pp.bin >= 0) {
+                resolve<T>(cl, src, n, base, w, true, goal, true, pp, [&](float l) {
+                    const int b = d_bin(l);
+                    return b >= b0 && b <= b1 && f_bin(l) == pp.bin;
+                });
                 cut = sh->cut;
             }
         }
     }
     const uint32_t cut_key = uint32_t(cut >> 32);
-    const float u = fminf(fmaxf(p.uniform[row], 0.f), 0.99999994f);
-    const int32_t token = locate(
-        cl, n, base,
-        [&](int i) -> u64 {
-            const float l = logit<T>(src, i);
-            const uint32_t key = key_of(l);
-            if (key < cut_key || ((u64(key) << 32) | (0xffffffffu - uint32_t(base + i))) < cut) return 0;
-            const u64 v = w(l);
-            return double(v) >= min_w ? v : 0;
-        },
-        [&](u64 total) { return double(u) * double(total); });
+    auto value = [&](int i, float l) -> u64 {
+        const uint32_t key = key_of(l);
+        if (key < cut_key || token_of(l, base + i) < cut) return 0;
+        const u64 v = w(l);
+        return double(v) >= min_w ? v : 0;
+    };
+    if (!summed) {
+        int s0, s1;
+        segment(n, warp, s0, s1);
+        each<T>(src + int64_t(s0) * es, s1 - s0, lane, 32, [&](int i, float l) { acc += value(s0 + i, l); });
+        acc = warp_sum64(acc);
+    }
+    const int32_t token =
+        find<T>(cl, src, n, base, acc, value, [&](u64 total) { return double(u) * double(total); });
     if (cl.rank == 0 && tid == 0) p.tokens[row] = token;
 }
 
 template <class T>
 cudaError_t run_sample(const Sample& p, cudaStream_t s) {
     const int sms = current_sm_count();
-    const size_t room = 227 * 1024 - sizeof(Shared);
-    // CTAs a row: enough to fill the GPU with few rows, at least 4096 tokens
-    // each, and enough to hold the row where eight can.
-    int C = 1;
+    const size_t room = 227 * 1024 - sizeof(Shared) - 16;  // (16: the row's own distance from a 16-byte border)
+    // CTAs a row: all SMs once with few rows, at least 4096 tokens each. (48 rows of 256000 f32: 3 CTAs, which read the
+    // row from L2 again, 120 us; 8, which hold it but are 2.6 waves, 189; 131 rows of 50257 f16: 1 CTA 20 us, 2 41 us; one
+    // row of 256000 bf16: 8 CTAs 22 us, 4 24, 1 44.)
     auto chunk_of = [&](int c) { return ((p.V + c - 1) / c + 7) / 8 * 8; };
-    while (C < 8 && ((p.rows * C * 2 <= sms && chunk_of(C) > 8192) || size_t(chunk_of(C)) * Elem<T>::bytes > room)) C *= 2;
+    int C = 1;
+    while (C < 8 && p.rows * (C + 1) <= sms && chunk_of(C) > 4096) ++C;
     const int64_t chunk = chunk_of(C);
     const bool resident = size_t(chunk) * Elem<T>::bytes <= room;
-    const size_t smem = sizeof(Shared) + (resident ? size_t(chunk) * Elem<T>::bytes : 0);
+    const size_t smem = sizeof(Shared) + (resident ? size_t(chunk) * Elem<T>::bytes + 16 : 0);
     static DeviceOnce once;
     cudaError_t e = once.run([] { return allow_smem(sample_kernel<T>, 227 * 1024); });
     if (e != cudaSuccess) return e;

@@ -216,3 +216,13 @@ def test_encoders_share_an_allocator():
     out, reused = ctypes.c_void_p(), ctypes.c_int()
     for st in (first, second):
         assert st.borrow(None, 64, ctypes.byref(out), ctypes.byref(reused)) == 0 and out.value == 4160
+
+
+def test_lengths_that_overflow_are_refused():
+    refused(E.tensorShapeMismatch, pc.Kernels.Sample, **sample_args(logits=fake([5, (1 << 21) + 1], D.bf16, 1 << 40)))
+    a = attention_args()
+    ps = a["k_pages"].shape[2]
+    W = (1 << 30) // ps
+    R = a["block_table"].shape[0]
+    pc.Kernels.PagedAttention(**dict(a, block_table=fake([R, W], ptr=1 << 30)))
+    refused(E.tensorShapeMismatch, pc.Kernels.PagedAttention, **dict(a, block_table=fake([R, W + 1], ptr=1 << 30)))

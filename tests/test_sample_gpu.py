@@ -189,3 +189,13 @@ def test_sample_unaligned_and_captured(pc, lib):
         torch.cuda.synchronize()
         xs = x.double().cpu().numpy()
         assert tokens.cpu().tolist() == [sample_plain(xs[r], now[r], p=0.9) for r in range(4)]
+
+
+def test_sample_largest_vocabulary(pc, lib):
+    """2^21 equal logits: their weights sum to 2^63."""
+    V = 1 << 21
+    x = torch.full((3, V), -1.5, dtype=torch.bfloat16, device="cuda")
+    u = np.array([0.0, 0.5, 0.75], np.float32)
+    assert draw(pc, lib, x, u).tolist() == [0, V // 2, V // 4 * 3]
+    assert draw(pc, lib, x, u, p=np.full(3, 0.5)).tolist() == [0, V // 4, V // 8 * 3]
+    assert draw(pc, lib, x, u, k=np.full(3, V // 2), p=np.full(3, 0.5)).tolist() == [0, V // 8, V // 16 * 3]
