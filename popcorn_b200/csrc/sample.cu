@@ -62,17 +62,17 @@ struct Pick {
 struct alignas(16) Shared {
     u64 mass[kBins], mass_all[kBins];  // (the second: sums over the cluster, in rank 0)
     uint32_t cnt[kBins], cnt_all[kBins];
-    double tab[32 * 16];  // 2^(j / 32), a copy a lane of a half-warp: no bank conflicts
+    double tab[64 * 16];  // 2^(j / 64), a copy a lane of a half-warp: no bank conflicts
     u64 wsum[32], wsum2[32];
     u64 ctot[8];
-    float cmax[8], cmin[8];
-    int32_t cidx[8];
     uint32_t ckmin[8], ckmax[8];
-    float fa[32], fb[32];
-    int32_t ia[32];
+    alignas(16) float maxima[8 * 32];
+    float minima[8 * 32];  // of all warps of the cluster
+    int32_t where[8 * 32];
+    float border;
     Pick pick;
     u64 cut, cut_mass;  // the last token of the prefix, and the prefix's weight
-    int lo_bin, hi_bin;
+    int lo_bin[2], hi_bin[2];
     uint32_t list_n;
     int32_t found;
     // (lists of candidates lie over the masses: 2048 keys, 2048 weights)
@@ -88,32 +88,51 @@ __device__ __forceinline__ float logit(const char* src, int i) {
     return tidy(Elem<T>::load(src, i));
 }
 
-// f(i, logit) for the n elements at src, 16 bytes at a time where alignment allows: thread `t` of `nt`.
+// f(i, l) for the n elements at src, by thread `t` of `nt`: l, an array, holds the logits (as they are) from the i-th on,
+// four at a time where alignment allows, so that their arithmetic overlaps. Loads run two rounds ahead of it: a row that does not stay in
+// shared memory comes from L2.
 template <class T, class F>
-__device__ __forceinline__ void each(const char* src, int n, int t, int nt, F f) {
+__device__ __forceinline__ void each4(const char* src, int n, int t, int nt, F f) {
     constexpr int es = Elem<T>::bytes, V = 16 / es;
     int head = int((16u - (uint32_t(reinterpret_cast<uintptr_t>(src)) & 15u)) & 15u) / es;
     head = head < n ? head : n;
     const int nv = (n - head) / V;
-    for (int i = t; i < head; i += nt) f(i, logit<T>(src, i));
+    auto one = [&](int i) {
+        const float l[1] = {Elem<T>::load(src, i)};
+        f(i, l);
+    };
+    for (int i = t; i < head; i += nt) one(i);
     const uint4* v = reinterpret_cast<const uint4*>(src + head * es);
-#pragma unroll 2
+    uint4 x = t < nv ? v[t] : uint4{}, y = t + nt < nv ? v[t + nt] : uint4{};
+#pragma unroll 1
     for (int c = t; c < nv; c += nt) {
-        const uint4 x = v[c];
+        const uint4 z = c + 2 * nt < nv ? v[c + 2 * nt] : uint4{};
         const int i = head + c * V;
         if constexpr (es == 4) {
-            f(i, tidy(__uint_as_float(x.x)));
-            f(i + 1, tidy(__uint_as_float(x.y)));
-            f(i + 2, tidy(__uint_as_float(x.z)));
-            f(i + 3, tidy(__uint_as_float(x.w)));
+            const float l[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
+            f(i, l);
         } else {
             float g[8];
             unpack8<T>(x, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f(i + e, tidy(g[e]));
+            const float l[4] = {g[0], g[1], g[2], g[3]};
+            f(i, l);
+            const float r[4] = {g[4], g[5], g[6], g[7]};
+            f(i + 4, r);
         }
+        x = y;
+        y = z;
     }
-    for (int i = head + nv * V + t; i < n; i += nt) f(i, logit<T>(src, i));
+    for (int i = head + nv * V + t; i < n; i += nt) one(i);
+}
+
+// f(i, logit), one at a time and tidy.
+template <class T, class F>
+__device__ __forceinline__ void each(const char* src, int n, int t, int nt, F f) {
+    each4<T>(src, n, t, nt, [&](int i, const auto& l) {
+        constexpr int N = sizeof(l) / sizeof(float);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(i + e, tidy(l[e]));
+    });
 }
 
 __device__ __forceinline__ uint32_t key_of(float f) {
@@ -129,33 +148,38 @@ __device__ __forceinline__ u64 token_of(float l, int32_t index) {
     return (u64(key_of(l)) << 32) | (0xffffffffu - uint32_t(index));
 }
 
+// The weight and the bin of a logit; l_max is finite. NaN compares false: it is not live.
 struct Weight {
-    float lmax, live;  // live: l_max - l above it weighs zero
-    double top, c32;   // l_max; 32 log2(e) / T
-    const double* tab;  // this lane's copy
+    float half_max, half_live;  // l_max / 2; half of what l_max - l may be (halves: their difference cannot overflow)
+    float scale;                // bins a unit of that half
+    double top, c64;            // l_max; 64 log2(e) / T
+    const double* tab;          // this lane's copy
 
-    __device__ __forceinline__ bool is_live(float l) const {
-        return l == lmax || (l > -INFINITY && lmax - l <= live);
+    __device__ __forceinline__ float half_below(float l) const { return fmaf(l, -0.5f, half_max); }
+    __device__ __forceinline__ bool is_live(float l) const { return half_below(l) <= half_live; }
+    // (2^23 is added: the nearest whole number, 0 .. kBins - 1 of a live token, is in the low bits)
+    __device__ __forceinline__ float raw_bin(float l) const { return fmaf(half_below(l), scale, 8388608.f); }
+    __device__ __forceinline__ int bin(float l) const {
+        return is_live(l) ? __float_as_int(raw_bin(l)) - 0x4b000000 : -1;
     }
-    // 2^42 exp((l - l_max) / T) to the nearest integer. With k = 32 log2 of the exponential and n the integer next to
-    // it: 2^(n / 32), from a table and an exponent, times 2^((k - n) / 32), |k - n| <= 1/2, by its series to the fifth
-    // power (the sixth is below 2^-48). Adding 1.5 2^52 or 2^52 leaves the nearest integer in a double's low bits.
-    __device__ __forceinline__ u64 operator()(float l) const {
-        if (l == lmax) return u64(1) << kOneBits;
-        const double k = (double(l) - top) * c32;
-        if (!(lmax - l <= live) || !(k >= -43.0 * 32.0)) return 0;
-        const double r = k + 6755399441055744.0;
+    // 2^42 exp((l - l_max) / T) of a live token, to the nearest integer. With k = 64 log2 of the exponential and n the
+    // integer next to it: 2^(n / 64), from a table and an exponent, times 2^((k - n) / 64), |k - n| <= 1/2, by its series
+    // to the fourth power (the fifth is below 2^-44). Adding 1.5 2^52 or 2^52 leaves the nearest integer in a double's low
+    // bits.
+    __device__ __forceinline__ u64 of_live(float l) const {
+        const double d = double(l) - top;
+        const double r = fma(d, c64, 6755399441055744.0);
         const int n = __double2loint(r);
-        const double x = k - (r - 6755399441055744.0);
-        double e = fma(x, 3.9737099845494154e-11, 9.172562701824643e-09);  // (ln 2 / 32)^i / i!
-        e = fma(e, x, 1.6938509724371819e-06);
-        e = fma(e, x, 2.3459619820224677e-04);
-        e = fma(e, x, 2.166084939249829e-02);
+        const double x = fma(d, c64, 6755399441055744.0 - r);
+        double e = fma(x, 5.732851688640402e-10, 2.1173137155464774e-07);  // (ln 2 / 64)^i / i!
+        e = fma(e, x, 5.864904955056169e-05);
+        e = fma(e, x, 1.0830424696249145e-02);
         e = fma(e, x, 1.0);
-        const double t = tab[(n & 31) * 16];
-        const double s = __hiloint2double(__double2hiint(t) + ((kOneBits + (n >> 5)) << 20), __double2loint(t));
+        const double t = tab[(n & 63) * 16];
+        const double s = __hiloint2double(__double2hiint(t) + ((kOneBits + (n >> 6)) << 20), __double2loint(t));
         return u64(__double_as_longlong(fma(e, s, 4503599627370496.0))) & ((u64(1) << 52) - 1);
     }
+    __device__ __forceinline__ u64 operator()(float l) const { return is_live(l) ? of_live(l) : 0; }
 };
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
@@ -584,40 +608,104 @@ __device__ u64 scan_cta(u64 v, u64& total, u64* wsum) {
     return incl + (warp ? wsum[warp - 1] : 0);
 }
 
-// The bins sh->lo_bin .. hi_bin in which the prefix of weight `goal` may end, from the counts alone: a bin's tokens weigh
-// between its borders' weights, half a unit each way for the weights' own rounding. (2^-16 of slack: of an exponent of at
-// most 29.9, l_max - l, the scale, their product and the border's exponent are each off by 2^-24 of it, exp2f by a little.)
-__device__ void end_bins(const Cluster& cl, double temp, float scale, double goal) {
+// The bins in which the prefix of weight `goal` may end, from the counts alone. [0]: for certain, as a bin's tokens weigh
+// between its borders' weights, half a unit each way for the weights' own rounding (2^-16 of slack: of an exponent of at
+// most 29.9, l_max - l, the scale, their product and the border's exponent are each off by 2^-24 of it, exp2f by a
+// little). [1]: a guess, where they weigh the mean of the two, and a bin more on both sides: a handful instead of what
+// holds 1.5 % of the weight.
+__device__ void end_bins(const Cluster& cl, double temp, const Weight& w, double goal) {
     Shared* sh = cl.sh;
     const int tid = threadIdx.x;
     if (cl.rank == 0) {
-        const double step = scale > 0.f ? 1.4426950408889634 / (temp * double(scale)) : 0.0;  // log2 a bin
+        const float scale = w.scale;
+        const double step = scale > 0.f ? 2.0 * 1.4426950408889634 / (temp * double(scale)) : 0.0;  // log2 a bin
         u64 hi[2], lo[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int b = 2 * tid + e;
             const double c = double(sh->cnt_all[b]);
-            hi[e] = u64(c * (kOne * double(exp2f(float(-step * b))) * (1.0 + 0x1p-16) + 0.5)) + 1;
-            lo[e] = scale > 0.f ? u64(c * fmax(kOne * double(exp2f(float(-step * (b + 1)))) * (1.0 - 0x1p-16) - 0.5, 0.0)) : 0;
+            hi[e] = u64(c * (kOne * double(exp2f(float(-step * fmax(b - 0.5, 0.0)))) * (1.0 + 0x1p-16) + 0.5)) + 1;
+            lo[e] = scale > 0.f ? u64(c * fmax(kOne * double(exp2f(float(-step * (b + 0.5)))) * (1.0 - 0x1p-16) - 0.5, 0.0)) : 0;
         }
-        if (tid == 0) sh->lo_bin = sh->hi_bin = kBins - 1;
-        u64 total;
-        const u64 th = scan_cta(hi[0] + hi[1], total, sh->wsum), tl = scan_cta(lo[0] + lo[1], total, sh->wsum2);
-        // the first bin with which the sum from above reaches the goal, and that from below
-        if (double(th) >= goal) atomicMin(&sh->lo_bin, double(th - hi[1]) >= goal ? 2 * tid : 2 * tid + 1);
-        if (double(tl) >= goal) atomicMin(&sh->hi_bin, double(tl - lo[1]) >= goal ? 2 * tid : 2 * tid + 1);
+        if (tid < 2) sh->lo_bin[tid] = sh->hi_bin[tid] = kBins - 1;
+        // the first bin with which the sum reaches the goal
+        auto first = [&](u64 x0, u64 x1, u64* wsum, int* out) {
+            u64 total;
+            const u64 t = scan_cta(x0 + x1, total, wsum);
+            if (double(t) >= goal) atomicMin(out, double(t - x1) >= goal ? 2 * tid : 2 * tid + 1);
+        };
+        first(hi[0], hi[1], sh->wsum, &sh->lo_bin[0]);
+        first(lo[0], lo[1], sh->wsum2, &sh->hi_bin[0]);
+        first(hi[0] / 2 + lo[0] / 2, hi[1] / 2 + lo[1] / 2, sh->wsum, &sh->lo_bin[1]);
         __syncthreads();
-        const int a = sh->lo_bin, b = sh->hi_bin;
-        if (tid < cl.C && tid > 0) {
-            cl.of(tid)->lo_bin = a;
-            cl.of(tid)->hi_bin = b;
+        const int a = sh->lo_bin[0], b = sh->hi_bin[0], g = sh->lo_bin[1];
+        __syncthreads();
+        if (tid < cl.C) {
+            Shared* o = cl.of(tid);
+            o->lo_bin[0] = a;
+            o->hi_bin[0] = b;
+            o->lo_bin[1] = g > 0 ? g - 1 : 0;
+            o->hi_bin[1] = g < kBins - 1 ? g + 1 : g;
         }
     }
     cl.sync();
 }
 
-// The token from a list of candidates (keys and indices) that holds the k first ones; one CTA.
-__device__ int32_t draw_from_list(Shared* sh, int n, int k, const Weight& w, float top_p, double min_w, float u) {
+// The token from a list of at most kCap candidates that holds the k first ones; one CTA. Four lanes a candidate, which
+// look at every other one twice: those before it in the order tell the cut, the kept ones of lower index the draw.
+__device__ int32_t draw_from_few(Shared* sh, int n, int k, const Weight& w, float top_p, u64 floor_w, float u) {
+    static_assert(4 * kCap <= kSampleThreads, "four lanes a candidate");
+    const int tid = threadIdx.x, i = tid >> 2, part = tid & 3;
+    const u64* list = sh->list();
+    u64* lw = sh->list_w();
+    const u64 me = i < n ? list[i] : 0;
+    const u64 v = i < n ? w(logit_of(uint32_t(me >> 32))) : 0;
+    if (part == 0) lw[i] = v;
+    if (tid == 0) sh->found = -1;
+    __syncthreads();
+    u64 above = 0;
+    int place = 0;
+    if (i - (i & 7) < n) {  // (whole warps)
+        for (int j = part; j < n; j += 4) {
+            const bool is = list[j] > me;
+            place += is;
+            above += is ? lw[j] : 0;
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            place += __shfl_xor_sync(0xffffffffu, place, o);
+            above += __shfl_xor_sync(0xffffffffu, above, o);
+        }
+    }
+    // (the last of the k knows the whole weight)
+    const bool in_k = i < n && place < k;
+    if (part == 0 && i < n && place == (n < k ? n : k) - 1) sh->cut_mass = above + v;
+    __syncthreads();
+    const double goal = top_p < 1.f ? fmax(double(top_p) * double(sh->cut_mass), 1.0) : 1e300;
+    const bool keep = in_k && double(above) < goal && v >= floor_w && v > 0;
+    if (part == 0) lw[i] = keep ? v : 0;
+    __syncthreads();
+    if (i - (i & 7) < n) {
+        u64 kept = 0, before = 0;
+        for (int j = part; j < n; j += 4) {
+            const u64 x = lw[j];
+            kept += x;
+            before += uint32_t(list[j]) > uint32_t(me) ? x : 0;  // (low words fall with the index)
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            kept += __shfl_xor_sync(0xffffffffu, kept, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        const double at = double(u) * double(kept);
+        if (keep && part == 0 && double(before) <= at && at < double(before + v)) sh->found = int32_t(0xffffffffu - uint32_t(me));
+    }
+    __syncthreads();
+    return sh->found;
+}
+
+// As draw_from_few, from up to kList candidates: sorted by the order, cut, sorted by index, drawn.
+__device__ int32_t draw_from_list(Shared* sh, int n, int k, const Weight& w, float top_p, u64 floor_w, float u) {
     const int tid = threadIdx.x;
     u64* list = sh->list();
     u64* lw = sh->list_w();
@@ -643,7 +731,7 @@ __device__ int32_t draw_from_list(Shared* sh, int n, int k, const Weight& w, flo
     for (int e = 0; e < 2; ++e) {
         const int i = 2 * tid + e;
         const u64 before = incl - v[1] - (e ? 0 : v[0]);
-        const bool keep = i < n && double(before) < goal && double(v[e]) >= min_w && v[e] > 0;
+        const bool keep = i < n && double(before) < goal && v[e] >= floor_w && v[e] > 0;
         // (the list's low words hold 2^32 - 1 - index: a larger one is an earlier token)
         const u64 id = keep ? (list[i] << 32) | uint32_t(i) : 0;
         lw[i] = keep ? v[e] : 0;
@@ -678,7 +766,9 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Cluster cl{sh, C, int(blockIdx.x % unsigned(C))};
     const int64_t row = blockIdx.x / unsigned(C);
-    if (tid < 512) sh->tab[tid] = exp2(double(tid >> 4) / 32.0);
+    if (tid == 0) sh->list_n = 0;
+    static_assert(kSampleThreads == 64 * 16, "an entry a thread");
+    sh->tab[tid] = exp2(double(tid >> 4) / 64.0);
     if (C > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // (this CTA runs)
     pdl_launch_dependents();
     pdl_wait();
@@ -690,6 +780,11 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
     char* data = smem + sizeof(Shared) + (reinterpret_cast<uintptr_t>(global) & 15u);
     const char* src = resident ? data : global;
 
+    const float temp = p.temperature ? p.temperature[row] : 1.f;
+    const int32_t k = p.top_k ? p.top_k[row] : 0;
+    const float tp = p.top_p ? p.top_p[row] : 1.f;
+    const float mp = p.min_p ? p.min_p[row] : 0.f;
+    const float u = fminf(fmaxf(p.uniform[row], 0.f), 0.99999994f);
     // the row's largest (and, for the histogram's range, smallest) logit
     float mx = -INFINITY, mn = INFINITY;
     int32_t mi = 0x7fffffff;
@@ -734,28 +829,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         each<T>(global, n, tid, kSampleThreads, look);
     }
     const float own = mx;  // this thread's largest
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, mx, o);
-        const int32_t oi = __shfl_xor_sync(0xffffffffu, mi, o);
-        if (om > mx || (om == mx && oi < mi)) {
-            mx = om;
-            mi = oi;
-        }
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    }
-    if (lane == 0) {
-        sh->fa[warp] = mx;
-        sh->fb[warp] = mn;
-        sh->ia[warp] = mi;
-    }
-    __syncthreads();
-    // every CTA of the cluster is running before its memory is written
-    if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (warp == 0) {
-        mx = sh->fa[lane];
-        mn = sh->fb[lane];
-        mi = sh->ia[lane];
+    auto reduce = [&] {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const float om = __shfl_xor_sync(0xffffffffu, mx, o);
@@ -766,80 +840,125 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
             }
             mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
         }
-        if (lane < C) {
-            Shared* o = cl.of(lane);
-            o->cmax[cl.rank] = mx;
-            o->cmin[cl.rank] = mn;
-            o->cidx[cl.rank] = mi;
-        }
+    };
+    reduce();
+    // every CTA of the cluster is running before its memory is written
+    if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (lane < C) {
+        Shared* o = cl.of(lane);
+        o->maxima[cl.rank * 32 + warp] = mx;
+        o->minima[cl.rank * 32 + warp] = mn;
+        o->where[cl.rank * 32 + warp] = mi;
     }
     cl.sync();
     mx = -INFINITY;
     mn = INFINITY;
     mi = 0x7fffffff;
     for (int r = 0; r < C; ++r) {
-        if (sh->cmax[r] > mx || (sh->cmax[r] == mx && sh->cidx[r] < mi)) {
-            mx = sh->cmax[r];
-            mi = sh->cidx[r];
+        const float om = sh->maxima[r * 32 + lane];
+        const int32_t oi = sh->where[r * 32 + lane];
+        if (om > mx || (om == mx && oi < mi)) {
+            mx = om;
+            mi = oi;
         }
-        mn = fminf(mn, sh->cmin[r]);
+        mn = fminf(mn, sh->minima[r * 32 + lane]);
     }
-    const float temp = p.temperature ? p.temperature[row] : 1.f;
+    reduce();
     if (!(temp > 0.f) || mx == -INFINITY) {  // (the same for the whole cluster)
         if (cl.rank == 0 && tid == 0) p.tokens[row] = mx == -INFINITY ? -1 : mi;
         return;  // no CTA touches another's memory after the barrier above
     }
-    const Weight w{mx, 29.9f * temp, double(mx), 32.0 * 1.4426950408889634 / double(temp), sh->tab + (lane & 15)};
-    const int32_t k = p.top_k ? p.top_k[row] : 0;
-    const float tp = p.top_p ? p.top_p[row] : 1.f;
-    const float mp = p.min_p ? p.min_p[row] : 0.f;
+    if (mx == INFINITY) {
+        // infinite logits weigh one each, the others nothing: the first k, the first p of them, all reach min-p
+        const int32_t token = locate<T>(
+            cl, src, n, base, [&](int, float l) { return u64(l == INFINITY ? 1 : 0); },
+            [&](u64 total) {
+                double take = k > 0 && double(k) < double(total) ? double(k) : double(total);
+                if (tp < 1.f) take = fmax(ceil(double(tp) * take), 1.0);
+                return double(u) * take;
+            });
+        if (cl.rank == 0 && tid == 0) p.tokens[row] = token;
+        return;
+    }
+    const float half_live = fminf(14.95f * temp, 3.402823466e38f);
+    const float half_range = fminf(fmaf(mn, -0.5f, 0.5f * mx), half_live);
+    const float bins = float(kBins - 1) / half_range;  // (a range too small for it: one bin)
+    const Weight w{0.5f * mx, half_live, bins <= 1e30f ? bins : 0.f,
+                   double(mx), 64.0 * 1.4426950408889634 / double(temp), sh->tab + (lane & 15)};
     const double min_w = mp > 0.f ? double(fminf(mp, 1.f)) * kOne : 0.0;
-    const float u = fminf(fmaxf(p.uniform[row], 0.f), 0.99999994f);
+    const u64 floor_w = u64(ceil(min_w));  // (v >= it as v >= min_w)
     const bool use_k = k > 0 && k < p.V, use_p = tp < 1.f;  // (NaN: off)
     u64 cut = 0;  // every token
     u64 acc = 0;  // the kept weight of this warp's segment
     bool summed = false;
     if (use_k || use_p) {
-        const float range = fminf(mx - mn, w.live);
-        const float scale = range > 0.f ? fminf(float(kBins) / range, 1e30f) : 0.f;
-        auto d_bin = [&](float l) {
-            if (!w.is_live(l)) return -1;
-            const float d = l == mx ? 0.f : mx - l;
-            const int b = int(d * scale);
-            return b < 0 ? 0 : (b >= kBins ? kBins - 1 : b);
-        };
+        auto d_bin = [&](float l) { return w.bin(l); };
         if (use_k && k <= kListK) {
-            // the border: from the threads' maxima, or from all tokens where those are too few to tell
-            const bool by_max = k <= kSampleThreads * C / 4;
-            Pick b;
-            if (by_max) {
-                clear_bins(cl, false);
-                const int at = d_bin(own);
-                if (at >= 0) atomicAdd(&sh->cnt[at], 1u);
-                gather_bins(cl, false);
-                b = pick_bin(cl, false, double(k), 0, 0);
-            }
-            if (!by_max || b.bin < 0) {
-                histogram<T>(cl, src, n, w, false, d_bin);
-                b = pick_bin(cl, false, double(k), 0, 0);
-            }
-            const int border = b.bin < 0 ? kBins - 1 : b.bin;
-            if (tid == 0) sh->list_n = 0;
-            cl.sync();
-            Shared* lead = cl.of(0);
-            const float end = border < kBins - 1 ? float(border + 1) : INFINITY;
-            each<T>(src, n, tid, kSampleThreads, [&](int i, float l) {
-                if (!((mx - l) * scale >= end) && w.is_live(l)) {  // (NaN: infinite logits)
-                    const uint32_t to = atomicAdd(&lead->list_n, 1u);
-                    if (to < kList) lead->list()[to] = token_of(l, base + i);
+            // a border that is not above the k-th largest logit: the k-th largest of the warps' maxima where there are
+            // four times as many (64 of 8 CTAs: 2 us against the histogram's 6), or the end of its bin among the
+            // threads' maxima, or among all tokens
+            float border = -INFINITY;
+            const int groups = 32 * C;
+            const bool own_ones = 4 * k <= kSampleThreads * C;
+            if (4 * k <= groups) {
+                // (four lanes a maximum, each with a fourth of the others; tid / 4 beyond them only helps its warp)
+                const int i = tid >> 2;
+                const float me = i < groups ? sh->maxima[i] : INFINITY;
+                int place = 0;
+                if (i - (i & 7) < groups)
+#pragma unroll 2
+                    for (int j = 4 * (tid & 3); j < groups; j += 16) {
+                        const float4 o = *reinterpret_cast<const float4*>(sh->maxima + j);
+                        place += o.x > me || (o.x == me && j < i);
+                        place += o.y > me || (o.y == me && j + 1 < i);
+                        place += o.z > me || (o.z == me && j + 2 < i);
+                        place += o.w > me || (o.w == me && j + 3 < i);
+                    }
+                place += __shfl_xor_sync(0xffffffffu, place, 1);
+                place += __shfl_xor_sync(0xffffffffu, place, 2);
+                if (i < groups && place == k - 1) sh->border = me;
+                __syncthreads();
+                border = sh->border;
+            } else {
+                Pick b;
+                b.bin = -1;
+                if (own_ones) {
+                    clear_bins(cl, false);
+                    const int at = d_bin(own);
+                    if (at >= 0) atomicAdd(&sh->cnt[at], 1u);
+                    gather_bins(cl, false);
+                    b = pick_bin(cl, false, double(k), 0, 0);
                 }
-            });
+                if (b.bin < 0) {
+                    histogram<T>(cl, src, n, w, false, d_bin);
+                    b = pick_bin(cl, false, double(k), 0, 0);
+                }
+                // (in logits: a little lower than the bin's end, whatever the roundings)
+                if (b.bin >= 0 && w.scale > 0.f)
+                    border = mx - 2.f * ((float(b.bin) + 0.5f) / w.scale) * 1.000001f - fabsf(mx) * 1e-6f;
+            }
+            Shared* lead = cl.of(0);
+            if (own >= border)  // (a thread's tokens are the same ones as when it took its maximum)
+                each4<T>(src, n, tid, kSampleThreads, [&](int i, const auto& l) {
+                    constexpr int N = sizeof(l) / sizeof(float);
+                    float most = l[0];
+#pragma unroll
+                    for (int e = 1; e < N; ++e) most = fmaxf(most, l[e]);
+                    if (!(most >= border)) return;
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (l[e] >= border && w.is_live(l[e])) {
+                            const uint32_t to = atomicAdd(&lead->list_n, 1u);
+                            if (to < kList) lead->list()[to] = token_of(tidy(l[e]), base + i + e);
+                        }
+                });
             cl.sync();
             const uint32_t found = lead->list_n;
             cl.sync();  // (the last look at another CTA's memory, if the list is complete)
             if (found <= kList) {
                 if (cl.rank == 0) {
-                    const int32_t token = draw_from_list(sh, int(found), k, w, tp, min_w, u);
+                    const int32_t token = found <= kCap ? draw_from_few(sh, int(found), k, w, tp, floor_w, u)
+                                                        : draw_from_list(sh, int(found), k, w, tp, floor_w, u);
                     if (tid == 0) p.tokens[row] = token;
                 }
                 return;
@@ -866,62 +985,104 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         }
         if (use_p) {
             clear_bins(cl, false);
-            const u64 all = total_of<T>(cl, src, n, [&](float l) -> u64 {
-                const int b = d_bin(l);
-                if (b < 0) return 0;
-                atomicAdd(&sh->cnt[b], 1u);
-                return whole ? w(l) : 0;
+            u64 all = 0;
+            each4<T>(src, n, tid, kSampleThreads, [&](int, const auto& l) {
+                constexpr int N = sizeof(l) / sizeof(float);
+                int b[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) b[e] = d_bin(l[e]);
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const u64 v = w.of_live(l[e]);
+                        all += b[e] >= 0 ? v : 0;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (b[e] >= 0) atomicAdd(&sh->cnt[b[e]], 1u);
             });
+            all = cluster_sum(cl, all);
             gather_bins(cl, false);
             if (whole) mass = double(all);
             const double goal = fmax(double(tp) * mass, 1.0);  // (p <= 0: the first token alone)
-            end_bins(cl, double(temp), scale, goal);
-            const int b0 = sh->lo_bin, b1 = sh->hi_bin;
-            // the weight before them exactly, and theirs by a 2048th of them; a warp's segment at a time, since the
-            // draw wants the kept weight of each
-            const float first = float(b0), fine = float(kBins) / float(b1 + 1 - b0);
+            // the bins it may end in: a guess first, which the sums prove or not, then the safe ones
+            end_bins(cl, double(temp), w, goal);
+            int b0, b1, s0, s1;
+            float first, fine;
             auto f_bin = [&](float l) {  // of a token in b0 .. b1: rises with l_max - l
-                const float f = l == mx ? 0.f : (mx - l) * scale;
-                const int b = int((f - first) * fine);
+                const int b = int(fmaf(w.half_below(l), w.scale, -first) * fine);
                 return b < 0 ? 0 : (b >= kBins ? kBins - 1 : b);
             };
-            int s0, s1;
             segment(n, warp, s0, s1);
             const char* part = src + int64_t(s0) * es;
-            clear_bins(cl, true);
-            u64 before = 0, kept = 0;
-            each<T>(part, s1 - s0, lane, 32, [&](int, float l) {
-                const int b = d_bin(l);
-                if (b < 0 || b > b1) return;
-                const u64 v = w(l);
-                if (b < b0) {
-                    before += v;
-                    if (double(v) >= min_w) kept += v;
-                    return;
-                }
-                const int f = f_bin(l);
-                atomicAdd(&sh->cnt[f], 1u);
-                if (v) atomicAdd(&sh->mass[f], v);
-            });
-            before = cluster_sum(cl, before);
-            gather_bins(cl, true);
-            const Pick pp = pick_bin(cl, true, goal, 0, before);
+            u64 kept;
+            Pick pp;
+#pragma unroll 1
+            for (int guess = 1; guess >= 0; --guess) {
+                b0 = sh->lo_bin[guess], b1 = sh->hi_bin[guess];
+                // the weight before them exactly, and theirs by a 2048th of them; a warp's segment at a time, since the
+                // draw wants the kept weight of each
+                first = float(b0) - 0.5f, fine = float(kBins) / float(b1 + 1 - b0);
+                const float f0 = 8388608.f + float(b0), f1 = 8388608.f + float(b1);
+                clear_bins(cl, true);
+                u64 before = 0;
+                kept = 0;
+                each4<T>(part, s1 - s0, lane, 32, [&](int, const auto& l) {
+                    constexpr int N = sizeof(l) / sizeof(float);
+                    bool in[N];
+                    u64 v[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const float f = w.raw_bin(l[e]);
+                        in[e] = f >= f0 && f <= f1;
+                        v[e] = w.of_live(l[e]);
+                        const u64 x = f < f0 ? v[e] : 0;  // (live: it is in an earlier bin than some)
+                        before += x;
+                        if (floor_w) kept += x >= floor_w ? x : 0;
+                    }
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (in[e] && w.is_live(l[e])) {
+                            const int f = f_bin(l[e]);
+                            atomicAdd(&sh->cnt[f], 1u);
+                            if (v[e]) atomicAdd(&sh->mass[f], v[e]);
+                        }
+                });
+                if (!floor_w) kept = before;
+                before = cluster_sum(cl, before);
+                gather_bins(cl, true);
+                pp = pick_bin(cl, true, goal, 0, before);
+                if (pp.bin >= 0) break;
+            }
             if (pp.bin >= 0 && pp.n <= kCap) {
                 // list the bin's tokens, and add to each segment's kept weight those before them
                 if (tid == 0) sh->list_n = 0;
                 cl.sync();
                 Shared* lead = cl.of(0);
-                each<T>(part, s1 - s0, lane, 32, [&](int i, float l) {
-                    const int b = d_bin(l);
-                    if (b < b0 || b > b1) return;
-                    const int f = f_bin(l);
-                    if (f < pp.bin) {
-                        const u64 v = w(l);
-                        if (double(v) >= min_w) kept += v;
-                    } else if (f == pp.bin) {
-                        const uint32_t at = atomicAdd(&lead->list_n, 1u);
-                        if (at < kCap) lead->list()[at] = token_of(l, base + s0 + i);
+                const float f0 = 8388608.f + float(b0), f1 = 8388608.f + float(b1);
+                each4<T>(part, s1 - s0, lane, 32, [&](int i, const auto& l) {
+                    constexpr int N = sizeof(l) / sizeof(float);
+                    bool in[N], any = false;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const float f = w.raw_bin(l[e]);
+                        in[e] = f >= f0 && f <= f1;
+                        any = any || in[e];
                     }
+                    if (!any) return;
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (in[e] && w.is_live(l[e])) {
+                            const int f = f_bin(l[e]);
+                            if (f < pp.bin) {
+                                const u64 v = w.of_live(l[e]);
+                                if (v >= floor_w) kept += v;
+                            } else if (f == pp.bin) {
+                                const uint32_t at = atomicAdd(&lead->list_n, 1u);
+                                if (at < kCap) lead->list()[at] = token_of(tidy(l[e]), base + s0 + i + e);
+                            }
+                        }
                 });
                 order_list(cl, w, true, goal, true, pp);
                 cut = sh->cut;
@@ -931,7 +1092,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
                     const int32_t at = int32_t(0xffffffffu - uint32_t(t)) - base;
                     if (t >= cut && at >= s0 && at < s1) {
                         const u64 v = w(logit_of(uint32_t(t >> 32)));
-                        if (double(v) >= min_w) kept += v;
+                        if (v >= floor_w) kept += v;
                     }
                 }
                 summed = true;
@@ -950,12 +1111,19 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         const uint32_t key = key_of(l);
         if (key < cut_key || token_of(l, base + i) < cut) return 0;
         const u64 v = w(l);
-        return double(v) >= min_w ? v : 0;
+        return v >= floor_w ? v : 0;
     };
     if (!summed) {
         int s0, s1;
         segment(n, warp, s0, s1);
-        each<T>(src + int64_t(s0) * es, s1 - s0, lane, 32, [&](int i, float l) { acc += value(s0 + i, l); });
+        each4<T>(src + int64_t(s0) * es, s1 - s0, lane, 32, [&](int i, const auto& l) {
+            constexpr int N = sizeof(l) / sizeof(float);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const u64 v = w.of_live(l[e]);
+                acc += w.is_live(l[e]) && v >= floor_w && token_of(tidy(l[e]), base + s0 + i + e) >= cut ? v : 0;
+            }
+        });
         acc = warp_sum64(acc);
     }
     const int32_t token =

@@ -199,3 +199,27 @@ def test_sample_largest_vocabulary(pc, lib):
     assert draw(pc, lib, x, u).tolist() == [0, V // 2, V // 4 * 3]
     assert draw(pc, lib, x, u, p=np.full(3, 0.5)).tolist() == [0, V // 4, V // 8 * 3]
     assert draw(pc, lib, x, u, k=np.full(3, V // 2), p=np.full(3, 0.5)).tolist() == [0, V // 8, V // 16 * 3]
+
+
+@pytest.mark.parametrize("V", [50, 40001])
+def test_sample_infinite_logits(pc, lib, V):
+    """+inf logits share all the weight, whatever stands beside them."""
+    x = bell(5, V, "f32", V)
+    x[:, 3::7] = float("inf")
+    x[:, 4] = torch.finfo(torch.float32).max
+    x[2, 5] = float("nan")
+    u = np.array([0.0, 0.3, 0.5, 0.8, 0.9999], np.float32)
+    for kw in ({}, dict(k=np.array([1, 2, 5, V // 7 + 3, V - 1])), dict(p=np.array([0.0, 1e-3, 0.5, 0.9, 1.0], np.float32)),
+               dict(k=np.full(5, V // 10), p=np.full(5, 0.37, np.float32), m=np.full(5, 1.0, np.float32))):
+        check(pc, lib, x, u, t=np.array([0.5, 1.0, 1e-30, 1e30, 2.0], np.float32), **kw)
+
+
+def test_sample_ranges_at_the_ends_of_f32(pc, lib):
+    """Differences that overflow, differences of a few of the smallest numbers, temperatures that go with them."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = torch.rand(4, 5000, generator=g, device="cuda") * 2 - 1
+    u = np.array([0.2, 0.4, 0.6, 0.8], np.float32)
+    for size, t in ((3.4e38, 3e38), (3.4e38, float("inf")), (1e-44, 1e-44), (1e-36, 1.0), (1e-30, 1e-30)):
+        x = r * size
+        for kw in ({}, dict(k=np.array([3, 1000, 4000, 4999])), dict(p=np.array([0.1, 0.5, 0.9, 0.99], np.float32))):
+            check(pc, lib, x, u, t=np.full(4, t, np.float32), **kw)
