@@ -61,23 +61,28 @@ struct Pick {
 
 struct alignas(16) Shared {
     u64 mass[kBins], mass_all[kBins];  // (the second: sums over the cluster, in rank 0)
-    uint32_t cnt[kBins], cnt_all[kBins];
-    double tab[64 * 16];  // 2^(j / 64), a copy a lane of a half-warp: no bank conflicts
+    alignas(16) uint32_t cnt[kBins];
+    uint32_t cnt_all[kBins];
+    // 2^(42 + j / 64) with j / 64 taken off the exponent's field, which n / 64 then adds; a copy a lane of a half-warp: no
+    // bank conflicts
+    double tab[64 * 16];
     u64 wsum[32], wsum2[32];
-    u64 ctot[8];
+    u64 ctot[8], ctot2[8];
+    u64 extra[32];  // of a warp's segment: the kept weight of the listed tokens
     uint32_t ckmin[8], ckmax[8];
     alignas(16) float maxima[8 * 32];
     float minima[8 * 32];  // of all warps of the cluster
-    int32_t where[8 * 32];
     float border;
     Pick pick;
     u64 cut, cut_mass;  // the last token of the prefix, and the prefix's weight
-    int lo_bin[2], hi_bin[2];
-    uint32_t list_n;
+    int lo_bin, hi_bin;
+    uint32_t list_n, local_n;
     int32_t found;
     // (lists of candidates lie over the masses: 2048 keys, 2048 weights)
     __device__ u64* list() { return mass; }
     __device__ u64* list_w() { return mass_all; }
+    // (and a CTA's own ones over the counts)
+    __device__ u64* local() { return reinterpret_cast<u64*>(cnt); }
 };
 
 // NaN counts as -inf, and -0 becomes +0: equal logits have equal keys.
@@ -162,11 +167,11 @@ struct Weight {
     __device__ __forceinline__ int bin(float l) const {
         return is_live(l) ? __float_as_int(raw_bin(l)) - 0x4b000000 : -1;
     }
-    // 2^42 exp((l - l_max) / T) of a live token, to the nearest integer. With k = 64 log2 of the exponential and n the
+    // 2^42 exp((l - l_max) / T) of a live token, to the nearest whole number. With k = 64 log2 of the exponential and n the
     // integer next to it: 2^(n / 64), from a table and an exponent, times 2^((k - n) / 64), |k - n| <= 1/2, by its series
-    // to the fourth power (the fifth is below 2^-44). Adding 1.5 2^52 or 2^52 leaves the nearest integer in a double's low
-    // bits.
-    __device__ __forceinline__ u64 of_live(float l) const {
+    // to the fourth power (the fifth is below 2^-44). Adding 1.5 2^52 or 2^52 rounds a double to a whole number. (A
+    // thread's share of a row, up to 2^11 of them, still sums exactly in a double.)
+    __device__ __forceinline__ double of_live(float l) const {
         const double d = double(l) - top;
         const double r = fma(d, c64, 6755399441055744.0);
         const int n = __double2loint(r);
@@ -176,10 +181,10 @@ struct Weight {
         e = fma(e, x, 1.0830424696249145e-02);
         e = fma(e, x, 1.0);
         const double t = tab[(n & 63) * 16];
-        const double s = __hiloint2double(__double2hiint(t) + ((kOneBits + (n >> 6)) << 20), __double2loint(t));
-        return u64(__double_as_longlong(fma(e, s, 4503599627370496.0))) & ((u64(1) << 52) - 1);
+        const double s = __hiloint2double(__double2hiint(t) + n * 16384, __double2loint(t));
+        return fma(e, s, 4503599627370496.0) - 4503599627370496.0;
     }
-    __device__ __forceinline__ u64 operator()(float l) const { return is_live(l) ? of_live(l) : 0; }
+    __device__ __forceinline__ u64 operator()(float l) const { return is_live(l) ? u64(of_live(l)) : 0; }
 };
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
@@ -307,6 +312,33 @@ __device__ u64 cluster_sum(const Cluster& cl, u64 acc) {
     return total;
 }
 
+// The sums of two, each thread's a whole number in a double.
+__device__ void cluster_sums(const Cluster& cl, double a, double b, u64& sum_a, u64& sum_b) {
+    Shared* sh = cl.sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 x = warp_sum64(u64(a)), y = warp_sum64(u64(b));
+    if (lane == 0) {
+        sh->wsum[warp] = x;
+        sh->wsum2[warp] = y;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        x = warp_sum64(sh->wsum[lane]);
+        y = warp_sum64(sh->wsum2[lane]);
+        if (lane < cl.C) {
+            cl.of(lane)->ctot[cl.rank] = x;
+            cl.of(lane)->ctot2[cl.rank] = y;
+        }
+    }
+    cl.sync();
+    sum_a = sum_b = 0;
+    for (int r = 0; r < cl.C; ++r) {
+        sum_a += sh->ctot[r];
+        sum_b += sh->ctot2[r];
+    }
+    cl.sync();
+}
+
 // value summed over the cluster's tokens, exactly.
 template <class T, class V>
 __device__ u64 total_of(const Cluster& cl, const char* src, int n, V value) {
@@ -357,6 +389,20 @@ __device__ void histogram(const Cluster& cl, const char* src, int n, const Weigh
         }
     });
     gather_bins(cl, masses);
+}
+
+// That of all tokens' counts.
+template <class T>
+__device__ void count_bins(const Cluster& cl, const char* src, int n, const Weight& w) {
+    Shared* sh = cl.sh;
+    clear_bins(cl, false);
+    each4<T>(src, n, threadIdx.x, kSampleThreads, [&](int, const auto& l) {
+        constexpr int N = sizeof(l) / sizeof(float);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (w.is_live(l[e])) atomicAdd(&sh->cnt[__float_as_int(w.raw_bin(l[e])) - 0x4b000000], 1u);
+    });
+    gather_bins(cl, false);
 }
 
 // The bin in which the prefix of `goal` ends: by count (the goal-th token) or by weight (the first token with which the
@@ -608,12 +654,12 @@ __device__ u64 scan_cta(u64 v, u64& total, u64* wsum) {
     return incl + (warp ? wsum[warp - 1] : 0);
 }
 
-// The bins in which the prefix of weight `goal` may end, from the counts alone. [0]: for certain, as a bin's tokens weigh
-// between its borders' weights, half a unit each way for the weights' own rounding (2^-16 of slack: of an exponent of at
-// most 29.9, l_max - l, the scale, their product and the border's exponent are each off by 2^-24 of it, exp2f by a
-// little). [1]: a guess, where they weigh the mean of the two, and a bin more on both sides: a handful instead of what
-// holds 1.5 % of the weight.
-__device__ void end_bins(const Cluster& cl, double temp, const Weight& w, double goal) {
+// The bins sh->lo_bin .. hi_bin in which the prefix of weight `goal` may end (or that of top_p times all weight, if goal is
+// negative), from the counts alone. A bin's tokens weigh between its borders' weights, half a unit each way for the weights'
+// own rounding (2^-16 of slack: of an exponent of at most 29.9, l_max - l, the scale, their product and the border's exponent
+// are each off by 2^-24 of it, exp2f by a little). A guess instead takes the mean of the two, and a bin more on both sides: a
+// handful of bins where the safe ones hold 1.5 % of the weight.
+__device__ void end_bins(const Cluster& cl, double temp, const Weight& w, double goal, double top_p, bool guess) {
     Shared* sh = cl.sh;
     const int tid = threadIdx.x;
     if (cl.rank == 0) {
@@ -626,29 +672,53 @@ __device__ void end_bins(const Cluster& cl, double temp, const Weight& w, double
             const double c = double(sh->cnt_all[b]);
             hi[e] = u64(c * (kOne * double(exp2f(float(-step * fmax(b - 0.5, 0.0)))) * (1.0 + 0x1p-16) + 0.5)) + 1;
             lo[e] = scale > 0.f ? u64(c * fmax(kOne * double(exp2f(float(-step * (b + 0.5)))) * (1.0 - 0x1p-16) - 0.5, 0.0)) : 0;
+            if (guess) hi[e] = lo[e] = hi[e] / 2 + lo[e] / 2;
         }
-        if (tid < 2) sh->lo_bin[tid] = sh->hi_bin[tid] = kBins - 1;
+        if (tid == 0) sh->lo_bin = sh->hi_bin = kBins - 1;
+        u64 total;
         // the first bin with which the sum reaches the goal
-        auto first = [&](u64 x0, u64 x1, u64* wsum, int* out) {
-            u64 total;
-            const u64 t = scan_cta(x0 + x1, total, wsum);
-            if (double(t) >= goal) atomicMin(out, double(t - x1) >= goal ? 2 * tid : 2 * tid + 1);
+        auto first = [&](u64 x0, u64 x1, int* out) {
+            const u64 t = scan_cta(x0 + x1, total, sh->wsum);
+            const double g = goal < 0.0 ? top_p * double(total) : goal;
+            if (double(t) >= g) atomicMin(out, double(t - x1) >= g ? 2 * tid : 2 * tid + 1);
         };
-        first(hi[0], hi[1], sh->wsum, &sh->lo_bin[0]);
-        first(lo[0], lo[1], sh->wsum2, &sh->hi_bin[0]);
-        first(hi[0] / 2 + lo[0] / 2, hi[1] / 2 + lo[1] / 2, sh->wsum, &sh->lo_bin[1]);
+        first(hi[0], hi[1], &sh->lo_bin);
+        if (!guess) first(lo[0], lo[1], &sh->hi_bin);
         __syncthreads();
-        const int a = sh->lo_bin[0], b = sh->hi_bin[0], g = sh->lo_bin[1];
+        int a = sh->lo_bin, b = sh->hi_bin;
+        if (guess) {
+            b = a < kBins - 1 ? a + 1 : a;
+            a = a > 0 ? a - 1 : 0;
+        }
         __syncthreads();
         if (tid < cl.C) {
             Shared* o = cl.of(tid);
-            o->lo_bin[0] = a;
-            o->hi_bin[0] = b;
-            o->lo_bin[1] = g > 0 ? g - 1 : 0;
-            o->hi_bin[1] = g < kBins - 1 ? g + 1 : g;
+            o->lo_bin = a;
+            o->hi_bin = b;
         }
     }
     cl.sync();
+}
+
+// The prefix's last token among n listed ones, `before` above them; one CTA. Sets sh->cut, or leaves it 0 if the goal lies
+// elsewhere.
+__device__ void cut_of_list(Shared* sh, int n, const Weight& w, u64 before, double goal) {
+    const int tid = threadIdx.x;
+    u64* list = sh->list();
+    int m = 64;
+    while (m < n) m <<= 1;
+    for (int i = n + tid; i < m; i += kSampleThreads) list[i] = 0;
+    if (tid == 0) sh->cut = 0;
+    sort_down(list, m);
+    u64 v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e] = 2 * tid + e < n ? w(logit_of(uint32_t(list[2 * tid + e] >> 32))) : 0;
+    u64 total;
+    const u64 incl = before + scan_cta(v[0] + v[1], total, sh->wsum);
+    const double p0 = double(incl - v[1] - v[0]), p1 = double(incl - v[1]), p2 = double(incl);
+    if (p0 < goal && goal <= p1) sh->cut = list[2 * tid];
+    if (p1 < goal && goal <= p2) sh->cut = list[2 * tid + 1];
+    __syncthreads();
 }
 
 // The token from a list of at most kCap candidates that holds the k first ones; one CTA. Four lanes a candidate, which
@@ -768,7 +838,10 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
     const int64_t row = blockIdx.x / unsigned(C);
     if (tid == 0) sh->list_n = 0;
     static_assert(kSampleThreads == 64 * 16, "an entry a thread");
-    sh->tab[tid] = exp2(double(tid >> 4) / 64.0);
+    {
+        const double t = exp2(double(tid >> 4) / 64.0);
+        sh->tab[tid] = __hiloint2double(__double2hiint(t) + (kOneBits << 20) - (tid >> 4) * 16384, __double2loint(t));
+    }
     if (C > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // (this CTA runs)
     pdl_launch_dependents();
     pdl_wait();
@@ -786,14 +859,11 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
     const float mp = p.min_p ? p.min_p[row] : 0.f;
     const float u = fminf(fmaxf(p.uniform[row], 0.f), 0.99999994f);
     // the row's largest (and, for the histogram's range, smallest) logit
+    // (fmaxf and fminf pass over NaN)
     float mx = -INFINITY, mn = INFINITY;
-    int32_t mi = 0x7fffffff;
-    auto look = [&](int i, float l) {
-        if (l > mx) {
-            mx = l;
-            mi = base + i;
-        }
-        if (l > -INFINITY) mn = fminf(mn, l);
+    auto look = [&](float l) {
+        mx = fmaxf(mx, l);
+        mn = fminf(mn, l);
     };
     if (resident) {
         int head = int((16u - (uint32_t(reinterpret_cast<uintptr_t>(global)) & 15u)) & 15u) / es;
@@ -802,7 +872,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         using S = typename T::storage;
         auto one = [&](int i) {
             reinterpret_cast<S*>(data)[i] = reinterpret_cast<const S*>(global)[i];
-            look(i, logit<T>(global, i));
+            look(Elem<T>::load(global, i));
         };
         if (tid < head) one(tid);
         const uint4* g = reinterpret_cast<const uint4*>(global + head * es);
@@ -811,33 +881,31 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         for (int c = tid; c < nv; c += kSampleThreads) {
             const uint4 x = g[c];
             d[c] = x;
-            const int i = head + c * V;
             if constexpr (es == 4) {
-                look(i, tidy(__uint_as_float(x.x)));
-                look(i + 1, tidy(__uint_as_float(x.y)));
-                look(i + 2, tidy(__uint_as_float(x.z)));
-                look(i + 3, tidy(__uint_as_float(x.w)));
+                look(__uint_as_float(x.x));
+                look(__uint_as_float(x.y));
+                look(__uint_as_float(x.z));
+                look(__uint_as_float(x.w));
             } else {
                 float f[8];
                 unpack8<T>(x, f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) look(i + e, tidy(f[e]));
+                for (int e = 0; e < 8; ++e) look(f[e]);
             }
         }
         if (tid < n - head - nv * V) one(head + nv * V + tid);
     } else {
-        each<T>(global, n, tid, kSampleThreads, look);
+        each4<T>(global, n, tid, kSampleThreads, [&](int, const auto& l) {
+            constexpr int N = sizeof(l) / sizeof(float);
+#pragma unroll
+            for (int e = 0; e < N; ++e) look(l[e]);
+        });
     }
     const float own = mx;  // this thread's largest
     auto reduce = [&] {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            const float om = __shfl_xor_sync(0xffffffffu, mx, o);
-            const int32_t oi = __shfl_xor_sync(0xffffffffu, mi, o);
-            if (om > mx || (om == mx && oi < mi)) {
-                mx = om;
-                mi = oi;
-            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
         }
     };
@@ -848,25 +916,22 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         Shared* o = cl.of(lane);
         o->maxima[cl.rank * 32 + warp] = mx;
         o->minima[cl.rank * 32 + warp] = mn;
-        o->where[cl.rank * 32 + warp] = mi;
     }
     cl.sync();
     mx = -INFINITY;
     mn = INFINITY;
-    mi = 0x7fffffff;
     for (int r = 0; r < C; ++r) {
-        const float om = sh->maxima[r * 32 + lane];
-        const int32_t oi = sh->where[r * 32 + lane];
-        if (om > mx || (om == mx && oi < mi)) {
-            mx = om;
-            mi = oi;
-        }
+        mx = fmaxf(mx, sh->maxima[r * 32 + lane]);
         mn = fminf(mn, sh->minima[r * 32 + lane]);
     }
     reduce();
+    mx += 0.f;  // (not -0)
     if (!(temp > 0.f) || mx == -INFINITY) {  // (the same for the whole cluster)
-        if (cl.rank == 0 && tid == 0) p.tokens[row] = mx == -INFINITY ? -1 : mi;
-        return;  // no CTA touches another's memory after the barrier above
+        const int32_t first = mx == -INFINITY ? -1
+                                              : locate<T>(cl, src, n, base, [&](int, float l) { return u64(l == mx ? 1 : 0); },
+                                                          [](u64) { return 0.0; });
+        if (cl.rank == 0 && tid == 0) p.tokens[row] = first;
+        return;
     }
     if (mx == INFINITY) {
         // infinite logits weigh one each, the others nothing: the first k, the first p of them, all reach min-p
@@ -881,7 +946,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         return;
     }
     const float half_live = fminf(14.95f * temp, 3.402823466e38f);
-    const float half_range = fminf(fmaf(mn, -0.5f, 0.5f * mx), half_live);
+    const float half_range = fminf(fmaf(mn, -0.5f, 0.5f * mx), half_live);  // (with -inf: half_live)
     const float bins = float(kBins - 1) / half_range;  // (a range too small for it: one bin)
     const Weight w{0.5f * mx, half_live, bins <= 1e30f ? bins : 0.f,
                    double(mx), 64.0 * 1.4426950408889634 / double(temp), sh->tab + (lane & 15)};
@@ -930,7 +995,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
                     b = pick_bin(cl, false, double(k), 0, 0);
                 }
                 if (b.bin < 0) {
-                    histogram<T>(cl, src, n, w, false, d_bin);
+                    count_bins<T>(cl, src, n, w);
                     b = pick_bin(cl, false, double(k), 0, 0);
                 }
                 // (in logits: a little lower than the bin's end, whatever the roundings)
@@ -968,7 +1033,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         double mass = 0.0;
         bool whole = true;  // top-k takes every token that weighs
         if (use_k) {
-            histogram<T>(cl, src, n, w, false, d_bin);
+            count_bins<T>(cl, src, n, w);
             Pick pk = pick_bin(cl, false, double(k), 0, 0);
             if (pk.bin >= 0) {
                 whole = false;
@@ -984,125 +1049,99 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
             }
         }
         if (use_p) {
-            clear_bins(cl, false);
-            u64 all = 0;
-            each4<T>(src, n, tid, kSampleThreads, [&](int, const auto& l) {
-                constexpr int N = sizeof(l) / sizeof(float);
-                int b[N];
-#pragma unroll
-                for (int e = 0; e < N; ++e) b[e] = d_bin(l[e]);
-                if (whole) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const u64 v = w.of_live(l[e]);
-                        all += b[e] >= 0 ? v : 0;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (b[e] >= 0) atomicAdd(&sh->cnt[b[e]], 1u);
-            });
-            all = cluster_sum(cl, all);
-            gather_bins(cl, false);
-            if (whole) mass = double(all);
-            const double goal = fmax(double(tp) * mass, 1.0);  // (p <= 0: the first token alone)
-            // the bins it may end in: a guess first, which the sums prove or not, then the safe ones
-            end_bins(cl, double(temp), w, goal);
-            int b0, b1, s0, s1;
-            float first, fine;
-            auto f_bin = [&](float l) {  // of a token in b0 .. b1: rises with l_max - l
-                const int b = int(fmaf(w.half_below(l), w.scale, -first) * fine);
-                return b < 0 ? 0 : (b >= kBins ? kBins - 1 : b);
-            };
+            count_bins<T>(cl, src, n, w);
+            double goal = whole ? -1.0 : fmax(double(tp) * mass, 1.0);  // (p <= 0: the first token alone)
+            int s0, s1;
             segment(n, warp, s0, s1);
             const char* part = src + int64_t(s0) * es;
-            u64 kept;
-            Pick pp;
-#pragma unroll 1
-            for (int guess = 1; guess >= 0; --guess) {
-                b0 = sh->lo_bin[guess], b1 = sh->hi_bin[guess];
-                // the weight before them exactly, and theirs by a 2048th of them; a warp's segment at a time, since the
-                // draw wants the kept weight of each
-                first = float(b0) - 0.5f, fine = float(kBins) / float(b1 + 1 - b0);
-                const float f0 = 8388608.f + float(b0), f1 = 8388608.f + float(b1);
-                clear_bins(cl, true);
-                u64 before = 0;
-                kept = 0;
-                each4<T>(part, s1 - s0, lane, 32, [&](int, const auto& l) {
-                    constexpr int N = sizeof(l) / sizeof(float);
-                    bool in[N];
-                    u64 v[N];
+            // a guess of the bins that the prefix ends in; all weight and that before them exactly, and their tokens listed
+            if (tid < 32) sh->extra[tid] = 0;
+            if (tid == 0) sh->list_n = sh->local_n = 0;
+            end_bins(cl, double(temp), w, goal, double(tp), true);
+            int b0 = sh->lo_bin, b1 = sh->hi_bin;
+            float f0 = 8388608.f + float(b0), f1 = 8388608.f + float(b1);
+            Shared* lead = cl.of(0);
+            double all = 0.0, first = 0.0, kept = 0.0;
+            const double min_weight = double(floor_w);
+            each4<T>(part, s1 - s0, lane, 32, [&](int i, const auto& l) {
+                constexpr int N = sizeof(l) / sizeof(float);
+                bool in[N], any = false;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float f = w.raw_bin(l[e]);
-                        in[e] = f >= f0 && f <= f1;
-                        v[e] = w.of_live(l[e]);
-                        const u64 x = f < f0 ? v[e] : 0;  // (live: it is in an earlier bin than some)
-                        before += x;
-                        if (floor_w) kept += x >= floor_w ? x : 0;
-                    }
+                for (int e = 0; e < N; ++e) {
+                    const float f = w.raw_bin(l[e]);
+                    const bool live = w.is_live(l[e]), early = f < f0;  // (an early one is live)
+                    in[e] = live && f >= f0 && f <= f1;
+                    any = any || in[e];
+                    const double v = w.of_live(l[e]);
+                    if (live) all += v;
+                    if (early) first += v;
+                    if (floor_w && early && v >= min_weight) kept += v;
+                }
+                if (!any) return;
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (in[e] && w.is_live(l[e])) {
-                            const int f = f_bin(l[e]);
-                            atomicAdd(&sh->cnt[f], 1u);
-                            if (v[e]) atomicAdd(&sh->mass[f], v[e]);
+                for (int e = 0; e < N; ++e)
+                    if (in[e]) {
+                        const u64 t = token_of(tidy(l[e]), base + s0 + i + e);
+                        const uint32_t at = atomicAdd(&sh->local_n, 1u);
+                        if (at < kList) {
+                            sh->local()[at] = t;
+                            const uint32_t to = atomicAdd(&lead->list_n, 1u);
+                            if (to < kList) lead->list()[to] = t;
+                        } else if (at == kList) {
+                            atomicAdd(&lead->list_n, uint32_t(kList));  // (too many)
                         }
-                });
-                if (!floor_w) kept = before;
-                before = cluster_sum(cl, before);
-                gather_bins(cl, true);
-                pp = pick_bin(cl, true, goal, 0, before);
-                if (pp.bin >= 0) break;
-            }
-            if (pp.bin >= 0 && pp.n <= kCap) {
-                // list the bin's tokens, and add to each segment's kept weight those before them
-                if (tid == 0) sh->list_n = 0;
+                    }
+            });
+            if (!floor_w) kept = first;
+            u64 total, before;
+            cluster_sums(cl, all, first, total, before);
+            if (whole) goal = fmax(double(tp) * double(total), 1.0);
+            bool done = false;
+            if (lead->list_n <= kList) {  // (the same for the whole cluster)
+                if (cl.rank == 0) {
+                    cut_of_list(sh, int(sh->list_n), w, before, goal);
+                    const u64 c = sh->cut;
+                    if (tid < C && tid > 0) cl.of(tid)->cut = c;
+                }
                 cl.sync();
-                Shared* lead = cl.of(0);
-                const float f0 = 8388608.f + float(b0), f1 = 8388608.f + float(b1);
-                each4<T>(part, s1 - s0, lane, 32, [&](int i, const auto& l) {
-                    constexpr int N = sizeof(l) / sizeof(float);
-                    bool in[N], any = false;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float f = w.raw_bin(l[e]);
-                        in[e] = f >= f0 && f <= f1;
-                        any = any || in[e];
-                    }
-                    if (!any) return;
-#pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (in[e] && w.is_live(l[e])) {
-                            const int f = f_bin(l[e]);
-                            if (f < pp.bin) {
-                                const u64 v = w.of_live(l[e]);
-                                if (v >= floor_w) kept += v;
-                            } else if (f == pp.bin) {
-                                const uint32_t at = atomicAdd(&lead->list_n, 1u);
-                                if (at < kCap) lead->list()[at] = token_of(tidy(l[e]), base + s0 + i + e);
-                            }
-                        }
-                });
-                order_list(cl, w, true, goal, true, pp);
+                done = sh->cut != 0;
+            }
+            if (done) {
                 cut = sh->cut;
-                // and of the listed ones those that are in the prefix
-                for (int j = lane; j < int(pp.n); j += 32) {
-                    const u64 t = lead->list()[j];
-                    const int32_t at = int32_t(0xffffffffu - uint32_t(t)) - base;
-                    if (t >= cut && at >= s0 && at < s1) {
-                        const u64 v = w(logit_of(uint32_t(t >> 32)));
-                        if (v >= floor_w) kept += v;
+                for (int i = tid; i < int(sh->local_n); i += kSampleThreads) {
+                    const u64 t = sh->local()[i];
+                    const u64 v = t >= cut ? w(logit_of(uint32_t(t >> 32))) : 0;
+                    if (v >= floor_w && v) {
+                        const int seg = ((n + 31) / 32 + 31) / 32 * 32;
+                        atomicAdd(&sh->extra[(int32_t(0xffffffffu - uint32_t(t)) - base) / seg], v);
                     }
                 }
+                __syncthreads();
                 summed = true;
-                acc = warp_sum64(kept);
-            } else if (pp.bin >= 0) {
-                resolve<T>(cl, src, n, base, w, true, goal, true, pp, [&](float l) {
+                acc = warp_sum64(u64(kept)) + sh->extra[warp];
+            } else {
+                // the safe bins; the weights of a 2048th of them each
+                cl.sync();
+                count_bins<T>(cl, src, n, w);
+                end_bins(cl, double(temp), w, goal, double(tp), false);
+                b0 = sh->lo_bin, b1 = sh->hi_bin;
+                const float start = float(b0) - 0.5f, fine = float(kBins) / float(b1 + 1 - b0);
+                auto f_bin = [&](float l) {  // of a token in b0 .. b1: rises with l_max - l
                     const int b = d_bin(l);
-                    return b >= b0 && b <= b1 && f_bin(l) == pp.bin;
+                    if (b < b0 || b > b1) return -1;
+                    const int f = int(fmaf(w.half_below(l), w.scale, -start) * fine);
+                    return f < 0 ? 0 : (f >= kBins ? kBins - 1 : f);
+                };
+                before = total_of<T>(cl, src, n, [&](float l) {
+                    const int b = d_bin(l);
+                    return b >= 0 && b < b0 ? w(l) : u64(0);
                 });
-                cut = sh->cut;
+                histogram<T>(cl, src, n, w, true, f_bin);
+                const Pick pp = pick_bin(cl, true, goal, 0, before);
+                if (pp.bin >= 0) {
+                    resolve<T>(cl, src, n, base, w, true, goal, true, pp, [&](float l) { return f_bin(l) == pp.bin; });
+                    cut = sh->cut;
+                }
             }
         }
     }
@@ -1114,17 +1153,19 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
         return v >= floor_w ? v : 0;
     };
     if (!summed) {
+        double sum = 0.0;
+        const double min_weight = double(floor_w);
         int s0, s1;
         segment(n, warp, s0, s1);
         each4<T>(src + int64_t(s0) * es, s1 - s0, lane, 32, [&](int i, const auto& l) {
             constexpr int N = sizeof(l) / sizeof(float);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const u64 v = w.of_live(l[e]);
-                acc += w.is_live(l[e]) && v >= floor_w && token_of(tidy(l[e]), base + s0 + i + e) >= cut ? v : 0;
+                const double v = w.of_live(l[e]);
+                if (w.is_live(l[e]) && v >= min_weight && (!cut || token_of(tidy(l[e]), base + s0 + i + e) >= cut)) sum += v;
             }
         });
-        acc = warp_sum64(acc);
+        acc = warp_sum64(u64(sum));
     }
     const int32_t token =
         find<T>(cl, src, n, base, acc, value, [&](u64 total) { return double(u) * double(total); });
