@@ -20,7 +20,8 @@ with the same rounding points:
     -> MatmulResidual (down_proj + Add)
 
 The position lives in device memory, so one captured CUDA graph serves
-every decode step.
+every decode step. PagedStack serves several requests at once over paged
+caches, prompts and decoding mixed, and draws the tokens.
 """
 from .api import AttentionMask, FixedScratch, KernelCommandEncoder, Kernels
 
@@ -282,6 +283,126 @@ class DecodeStack:
     def algorithmic_bytes_per_step(self, ctx):
         lm = self.vocab * self.shape.H * _nbytes(self.x) // self.x.numel() if self.vocab else 0
         return len(self.layers) * self.shape.bytes_per_token(ctx) + lm
+
+
+class PagedStack:
+    """A stack of decode layers that serves up to `requests` requests at once
+    over paged K/V caches: one step takes up to `tokens` new tokens, one of a
+    request that decodes, a chunk of a prompt, or none, and draws the next
+    token of every request.
+
+        PagedBatchBuild -> EmbeddingGather, RopeBuildCosSin
+        per layer: RMSNorm (or the AddRMSNorm before) -> Matmul [q; k; v]
+            -> PagedQKVScatter (norms, RoPE, into the pages)
+            -> PagedAttention -> Matmul (o) -> AddRMSNorm
+            -> Matmul [gate; up] -> GatedActivation -> Matmul (down)
+            -> AddRMSNorm
+        the requests' last rows -> Matmul (LM head) -> Sample
+
+    A step reads `added` [requests] (new tokens each), `ids` [tokens] (their
+    token ids, request after request), `uniform` [requests] (numbers in
+    [0, 1)) and the sampling parameters `temperature`, `top_k`, `top_p` and
+    `min_p` [requests]; it keeps `seq_lens`, `block_table` and `free_head` on
+    the device, and leaves `logits` [requests, vocab], `next` [requests] and
+    `admitted`, the number of requests, from the first on, that fitted. The
+    others wait: their lengths stay, and their logits and tokens mean
+    nothing, nor do those of a request without new tokens. All shapes are
+    fixed, so that one captured graph serves every step. The caller writes
+    free page ids to `free_pages` and moves `free_head` when it gets pages
+    back."""
+
+    def __init__(self, library, shape, n_layers, vocab, requests, tokens, pages, page_size=64, seed=0, device=0,
+                 rope_theta=10000.0, norm_add_one=True, qk_norm=True, mask=AttentionMask.causal, sinks=0):
+        """`shape.Smax` bounds a request's length (the block table's width)."""
+        import torch
+        s = shape
+        dev = "cuda:%d" % device
+        tdt = _torch_dtype(s.dtype)
+        self.shape, self.library, self.vocab = shape, library, vocab
+        self.requests, self.tokens, self.page_size = requests, tokens, page_size
+        self.norm_add_one, self.qk_norm, self.mask, self.sinks = norm_add_one, qk_norm, mask, sinks
+        g = torch.Generator(device=dev).manual_seed(seed)
+        small = LayerShape(s.H, s.Nq, s.Nkv, s.Hd, s.F, 1, s.dtype)  # (the weights; their caches are not used)
+        self.layers = []
+        for _ in range(n_layers):
+            w = DecodeLayerWeights(small, g, device=dev)
+            w.w_gate_up = torch.cat([w.w_gate, w.w_up])
+            del w.w_gate, w.w_up, w.k_cache, w.v_cache
+            w.q_norm, w.k_norm = [(torch.randn(s.Hd, generator=g, device=dev) * 0.1).float() for _ in range(2)]
+            w.k_pages = torch.zeros(pages, s.Nkv, page_size, s.Hd, dtype=tdt, device=dev)
+            w.v_pages = torch.zeros_like(w.k_pages)
+            self.layers.append(w)
+        self.final_norm = (torch.randn(s.H, generator=g, device=dev) * 0.1).float()
+        self.embedding = (torch.randn(vocab, s.H, generator=g, device=dev) * 0.02).to(tdt)  # (and the LM head)
+        self.inv_freq = (rope_theta ** (-torch.arange(0, s.Hd, 2, dtype=torch.float32) / s.Hd)).to(dev)
+
+        def i32(*shape):
+            return torch.zeros(*shape, dtype=torch.int32, device=dev)
+
+        def act(*shape):
+            return torch.zeros(*shape, dtype=tdt, device=dev)
+
+        R, T = requests, tokens
+        # the step's inputs, the state and the results
+        self.added, self.ids = i32(R), i32(T)
+        self.uniform = torch.zeros(R, device=dev)
+        self.temperature, self.top_p, self.min_p = torch.ones(R, device=dev), torch.ones(R, device=dev), torch.zeros(R, device=dev)
+        self.top_k = i32(R)
+        self.free_pages = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.free_head = i32(1)
+        self.block_table = i32(R, (s.Smax + page_size - 1) // page_size)
+        self.seq_lens, self.query_start, self.last_rows, self.admitted = i32(R), i32(R + 1), i32(R), i32(1)
+        self.positions, self.slots = i32(T), i32(T)
+        self.logits, self.next = act(R, vocab), i32(R)
+        # activations
+        self.cos = torch.zeros(T, s.Hd // 2, device=dev)
+        self.sin = torch.zeros_like(self.cos)
+        self.x, self.h, self.xn, self.part = act(T, s.H), act(T, s.H), act(T, s.H), act(T, s.H)
+        self.qkv = act(T, (s.Nq + 2 * s.Nkv) * s.Hd)
+        self.q, self.attn = act(T, s.Nq, s.Hd), act(T, s.Nq, s.Hd)
+        self.gate_up, self.act = act(T, 2 * s.F), act(T, s.F)
+        self.last = act(R, s.H)
+        self.scratch = FixedScratch(96 << 20, device)
+        self._kernels = None
+
+    def kernels(self):
+        """The validated kernel objects of one step (built once)."""
+        if self._kernels is not None:
+            return self._kernels
+        s, K, T = self.shape, Kernels, self.tokens
+        norm = dict(eps=s.eps, add_one_to_weight=self.norm_add_one)
+        ks = [K.PagedBatchBuild(self.seq_lens, self.added, self.free_pages, self.free_head, self.block_table,
+                                self.page_size, self.seq_lens, self.query_start, self.positions, self.slots,
+                                self.last_rows, self.free_head, self.admitted),
+              K.EmbeddingGather(self.ids, self.embedding, self.x),
+              K.RopeBuildCosSin(self.positions, self.inv_freq, self.cos, self.sin, 1.0),
+              K.RMSNorm(self.x, self.layers[0].attn_norm, into=self.xn, **norm)]
+        for i, w in enumerate(self.layers):
+            after = self.layers[i + 1].attn_norm if i + 1 < len(self.layers) else self.final_norm
+            ks += [K.Matmul(self.xn, w.w_qkv, into=self.qkv, transpose_b=True),
+                   K.PagedQKVScatter(self.qkv, self.slots, self.q, w.k_pages, w.v_pages, self.cos, self.sin,
+                                     qk_norm=self.qk_norm, q_norm=w.q_norm if self.qk_norm else None,
+                                     k_norm=w.k_norm if self.qk_norm else None, norm_v=self.qk_norm, **norm),
+                   K.PagedAttention(self.q, w.k_pages, w.v_pages, self.block_table, self.seq_lens, self.query_start,
+                                    into=self.attn, scale=s.scale, mask=self.mask, sinks=self.sinks),
+                   K.Matmul(self.attn.view(T, s.Nq * s.Hd), w.w_o, into=self.part, transpose_b=True),
+                   K.AddRMSNorm(self.x, self.part, w.mlp_norm, self.h, self.xn, **norm),
+                   K.Matmul(self.xn, w.w_gate_up, into=self.gate_up, transpose_b=True),
+                   K.GatedActivation(self.gate_up, self.act, s.activation),
+                   K.Matmul(self.act, w.w_down, into=self.part, transpose_b=True),
+                   K.AddRMSNorm(self.h, self.part, after, self.x, self.xn, **norm)]
+        ks += [K.EmbeddingGather(self.last_rows, self.xn, self.last),
+               K.Matmul(self.last, self.embedding, into=self.logits, transpose_b=True),
+               K.Sample(self.logits, self.uniform, self.next, self.temperature, self.top_k, self.top_p, self.min_p)]
+        self._kernels = ks
+        return ks
+
+    def encoder(self, stream=None):
+        return KernelCommandEncoder(self.library, stream=stream, scratch=self.scratch)
+
+    def encode_step(self, encoder):
+        encoder.encode(*self.kernels())
+        return self.next
 
 
 class AqLayerWeights:
