@@ -788,7 +788,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         Walk walk(a, s_plan);
         bool ok = true;
         const int box_keys = a.box_groups * 8;
-        const int per_fill = 32 / boxes;  // units whose boxes one look at the table covers
+        // units whose boxes one look at the table covers (fewer than there are notes: they are waited for at once)
+        const int per_fill = boxes < 8 ? 4 : 32 / boxes;
+        static_assert(kNotes > 4, "a look's notes fit the ring");
         const int my_unit = lane / boxes, my_box = lane % boxes;
         // The page of this lane's box, of unit u + my_unit (-1: no row sees a key of it). Read ahead: the table's
         // latency is longer than a tile's loads take to issue.
@@ -828,23 +830,29 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 nu = nx.u0;
             }
             if (more) page = page_of(nx, nu);
+            // each unit's flags, by its lanes
+            const int mine = u_first + my_unit, tile = tile_of(it, mine), key0 = tile * kN;
+            int flags = (mine == it.u0 ? kFirst : 0) | (mine == it.u1 - 1 ? kLast : 0) |
+                        (keys_open(a, it, key0, kN) ? kOpen : 0);
+            if (mine + 1 < it.u1) flags |= mine + 2 == it.u1 ? kNextLast : 0;
+            else flags |= !more ? kNextStop : (kNextFirst | (nx.u0 + 1 == nx.u1 ? kNextLast : 0));
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                if (!(flags & kOpen) && guarded(a, it, key0 + h * S::KEYS, S::KEYS)) flags |= kLook << h;
+            // (warp 3 hands notes back in order and needs nothing from here for those of units before j)
+            const int j_end = j + (u_end - u_first) - 1;
+            ok = wait_bar(unit_free[j_end % kNotes], (uint32_t(j_end / kNotes) & 1u) ^ 1u, s_abort);
             for (int u = u_first; u < u_end && ok; ++u, ++j) {
                 Unit& note = s_unit[j % kNotes];
-                ok = wait_bar(unit_free[j % kNotes], (uint32_t(j / kNotes) & 1u) ^ 1u, s_abort);
-                if (!ok) break;
-                if (my_unit == u - u_first) note.group[my_box] = g;
+                if (my_unit == u - u_first) {
+                    note.group[my_box] = g;
+                    if (my_box == 0) {
+                        note.flags = flags;
+                        note.tile = tile;
+                    }
+                }
                 __syncwarp();
                 if (lane == 0) {
-                    const int key0 = tile_of(it, u) * kN;
-                    int flags = (u == it.u0 ? kFirst : 0) | (u == it.u1 - 1 ? kLast : 0) |
-                                (keys_open(a, it, key0, kN) ? kOpen : 0);
-                    if (u + 1 < it.u1) flags |= u + 2 == it.u1 ? kNextLast : 0;
-                    else flags |= !more ? kNextStop : (kNextFirst | (nx.u0 + 1 == nx.u1 ? kNextLast : 0));
-                    note.tile = tile_of(it, u);
-#pragma unroll
-                    for (int h = 0; h < H; ++h)
-                        if (!(flags & kOpen) && guarded(a, it, key0 + h * S::KEYS, S::KEYS)) flags |= kLook << h;
-                    note.flags = flags;
                     if (u == it.u0) {
                         s_poison[items % kNotes] = 0;
                         s_item[items % kNotes] = it;
