@@ -789,8 +789,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         bool ok = true;
         const int box_keys = a.box_groups * 8;
         // units whose boxes one look at the table covers (fewer than there are notes: they are waited for at once)
-        const int per_fill = boxes < 8 ? 4 : 32 / boxes;
-        static_assert(kNotes > 4, "a look's notes fit the ring");
+        const int per_fill = boxes < 32 / (kNotes - 1) ? kNotes - 1 : 32 / boxes;
         const int my_unit = lane / boxes, my_box = lane % boxes;
         // The page of this lane's box, of unit u + my_unit (-1: no row sees a key of it). Read ahead: the table's
         // latency is longer than a tile's loads take to issue.
