@@ -483,20 +483,20 @@ PC_API int pc_kernel_paged_qkv_scatter(const pc_tensor* qkv, const pc_tensor* sl
  * keys: causal j <= position; sliding window also position - j < window, or
  * j < sinks (the first `sinks` tokens stay visible; sinks > 0 only with that
  * mask); bidirectional all. KV head hq * Nkv / Nq, Hd <= 512, at most 2^30
- * keys a request, one float dtype. fp32 softmax and accumulation; a row without a visible key is zero;
- * rows of no request are left as they are. Values in keys that a row does
- * not see never reach it, whatever they are. Lengths are clamped to the
- * tensors on the device; a page id outside the pages is never read: it sets
- * bit 5 of the device error word and its request's rows hold no meaningful
- * result. */
+ * keys a request, one float dtype. fp32 softmax and accumulation; a row
+ * without a visible key is zero; rows of no request are left as they are.
+ * Values in keys that a row does not see never reach it, whatever they are.
+ * Lengths are clamped to the tensors on the device; a page id outside the
+ * pages is never read: it sets bit 5 of the device error word and its
+ * request's rows hold no meaningful result. */
 PC_API int pc_kernel_paged_attention(const pc_tensor* q, const pc_tensor* k_pages, const pc_tensor* v_pages,
                                      const pc_tensor* block_table, const pc_tensor* seq_lens,
                                      const pc_tensor* query_start, const pc_tensor* out, float scale,
                                      pc_attention_mask mask, int32_t sinks, pc_kernel** kernel);
 /* The next token of each row of logits [.., V] (f32, f16, bf16; V <= 2^21)
- * from one given random number uniform [rows] in [0, 1), f32. With w_i = exp((l_i -
- * l_max) / temperature) and tokens ordered by (logit descending, index
- * ascending): top_k (i32; <= 0 or >= V: off) keeps the first k; top_p (f32;
+ * from one given random number uniform [rows] in [0, 1), f32. With w_i =
+ * exp((l_i - l_max) / temperature) and tokens ordered by (logit descending,
+ * index ascending): top_k (i32; <= 0 or >= V: off) keeps the first k; top_p (f32;
  * >= 1 or NaN: off) the shortest prefix of those whose weight reaches top_p
  * times theirs, one at least; min_p (f32; <= 0 or NaN: off) those with w_i
  * >= min(min_p, 1). The token is the first index, in index order, at which

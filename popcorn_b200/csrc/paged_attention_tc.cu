@@ -19,13 +19,26 @@
 // one ring in the order K(0), K(1), V(0), K(2), V(1), ...; warp 1 issues S = Q.K^T
 // into the next of NS accumulators in tensor memory, warp 12 O += P.V (one
 // issuer for both spent half of its time in looking at barriers, some 150
-// clocks each: 2430 instead of 1700 clocks a tile at Hd 128); warps 4-7 and 8-11 take tiles in turn (a thread a row) and turn S
-// into P = 2^(c S - m): P is packed into the type and written back over S,
-// from where the second product reads it as its A operand, so it never passes
-// through shared memory; one group's loads and waits pass under the other's
-// exponentials (the MUFU's 16 a clock are the bound: 1024 clocks a tile). A ring slot holds 8-key groups of [Hd/64][8 keys][128 B], so
-// any page size that is a multiple of 8 gives one layout (group stride Hd/64
-// KB) and the two halves of a tile in neighbouring slots are one operand.
+// clocks each: 2430 instead of 1700 clocks a tile at Hd 128); warps 4-7 and
+// 8-11 take tiles in turn (a thread a row) and turn S into P = 2^(c S - m): P
+// is packed into the type and written back over S, from where the second
+// product reads it as its A operand, so it never passes through shared
+// memory; one group's loads and waits pass under the other's exponentials. A
+// ring slot holds 8-key groups of [Hd/64][8 keys][128 B], so any page size
+// that is a multiple of 8 gives one layout (group stride Hd/64 KB) and the two
+// halves of a tile in neighbouring slots are one operand.
+//
+// What bounds it. Decoding: HBM; 32 requests of up to 8192 keys, 8 KV heads
+// of 256: 216 us in a row (5.3 TB/s), 250 with cold lengths and tables; a
+// single request of 4096 keys is all latency (27 us: plan 5, first tiles 8,
+// join 4). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
+// tile) nor the tensor cores (as many), but the chain product, look at a
+// barrier, softmax, product of a tile, some 6700 clocks, over the NS tiles in
+// flight: 2250 clocks a tile at Hd 128 (32 % of the tensor cores' time; a
+// window of 4096 and 4 sinks, 2000 tokens of 32 heads: 210 us, 623 TFLOP/s of
+// visible pairs' work). Tiles of 64 keys, twice as many in flight, cost the
+// loads' warp as much each as those of 128: 315 us. Holding a half of S in
+// registers over the wait for the max spills: 250 us.
 //
 // The running max is kept until it grows by more than 2^8 (P <= 256 then; O
 // and l use the same max, so O / l is exact for any); it goes from group to
