@@ -30,8 +30,8 @@
 //
 // What bounds it. Decoding: HBM; 32 requests of up to 8192 keys, 8 KV heads
 // of 256: 216 us in a row (5.3 TB/s), 250 with cold lengths and tables; a
-// single request of 4096 keys is all latency (27 us: plan 5, first tiles 8,
-// join 4). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
+// single request of 4096 keys is all latency (27 us; a CTA's first product
+// comes some 12 us after its start: plan 7, look-ups and loads 5). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
 // tile) nor the tensor cores (as many), but the chain product, look at a
 // barrier, softmax, product of a tile, some 6700 clocks, over the NS tiles in
 // flight: 2250 clocks a tile at Hd 128 (32 % of the tensor cores' time; a

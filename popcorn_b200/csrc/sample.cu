@@ -18,7 +18,7 @@
 // One cluster of up to eight CTAs per row: the row is read from HBM once and
 // stays in the CTAs' shared memory if it fits (else it is read again from
 // L2). Nothing is sorted but a few candidates:
-//  * top-k up to 1024: a logit that is not above the k-th largest is the k-th
+//  * top-k up to 512: a logit that is not above the k-th largest is the k-th
 //    largest of the maxima of many groups of tokens (the warps', or, by a
 //    histogram, the threads'). The tokens from it on, hardly more than k, go
 //    to one CTA, which does all the rest.
@@ -36,7 +36,7 @@
 // Bound by instructions and, with few rows, by the chain of cluster barriers
 // (some 0.6 us each) and cold code; the HBM floor is far. One row of 256000
 // bf16, top-k 64: 11 us (all sorting and histogramming in full: 58). 131 rows
-// of 50257 f16, top-k 200: 19 us. 48 rows of 256000 f32, top-p 0.9: 78 us, 95
+// of 50257 f16, top-k 200: 18 us. 48 rows of 256000 f32, top-p 0.9: 78 us, 95
 // when the 49 MB come from HBM (a pass of weights more: 120; weights by exp():
 // 250).
 #include <cooperative_groups.h>
@@ -58,7 +58,12 @@ constexpr int kSampleThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kCap = 256;     // tokens of a bin that are ordered directly
 constexpr int kList = 2048;   // candidates of a small top-k
-constexpr int kListK = 1024;  // the largest such k
+// The largest such k: 131 rows of 50257 f16, one of 256000 bf16, 64 of 32000 f32 take 24, 23 and 21 us with the list at k =
+// 400 and 30, 38 and 26 us at 1000; by the histogram of all tokens 32, 29 and 20 us whatever k is.
+constexpr int kListK = 512;
+// Candidates that are drawn by looking at each pair; more are sorted (k = 100, so hardly more candidates: 12.1, 15.9 and
+// 14.2 us against 15.2, 18.9 and 16.9; k = 200: 18.3, 20.3 and 18.9 against 17.5, 20.3 and 18.7).
+constexpr int kFew = 192;
 constexpr int kOneBits = 42;
 constexpr double kOne = 4398046511104.0;  // 2^42
 
@@ -731,10 +736,10 @@ __device__ void cut_of_list(Shared* sh, int n, const Weight& w, u64 before, doub
     __syncthreads();
 }
 
-// The token from a list of at most kCap candidates that holds the k first ones; one CTA. Four lanes a candidate, which
+// The token from a list of at most kFew candidates that holds the k first ones; one CTA. Four lanes a candidate, which
 // look at every other one twice: those before it in the order tell the cut, the kept ones of lower index the draw.
 __device__ int32_t draw_from_few(Shared* sh, int n, int k, const Weight& w, float top_p, u64 floor_w, float u) {
-    static_assert(4 * kCap <= kSampleThreads, "four lanes a candidate");
+    static_assert(4 * kFew <= kSampleThreads, "four lanes a candidate");
     const int tid = threadIdx.x, i = tid >> 2, part = tid & 3;
     const u64* list = sh->list();
     u64* lw = sh->list_w();
@@ -1032,7 +1037,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const Sample 
             cl.sync();  // (the last look at another CTA's memory, if the list is complete)
             if (found <= kList) {
                 if (cl.rank == 0) {
-                    const int32_t token = found <= kCap ? draw_from_few(sh, int(found), k, w, tp, floor_w, u)
+                    const int32_t token = found <= kFew ? draw_from_few(sh, int(found), k, w, tp, floor_w, u)
                                                         : draw_from_list(sh, int(found), k, w, tp, floor_w, u);
                     if (tid == 0) p.tokens[row] = token;
                 }
