@@ -47,9 +47,15 @@ bool overlap(const Tensor& a, const Tensor& b) {
     return nx && ny && x < y + ny && y < x + nx;
 }
 
-// Every output apart from every other tensor, except the pairs in `same`
-// (which may be one buffer, whole).
+// Every tensor at an address of its type's alignment; every output apart
+// from every other tensor, except the pairs in `same` (which may be one
+// buffer, whole).
 void apart(const std::vector<Binding>& bindings, const char* what, const std::vector<std::pair<size_t, size_t>>& same = {}) {
+    for (const Binding& b : bindings) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(b.tensor.data());
+        want(b.tensor.element_count() == 0 || (at && at % uintptr_t(dtype_stride(b.tensor.dtype())) == 0),
+             PC_ERR_TENSOR_SHAPE_MISMATCH, std::string(what) + " has a tensor without memory, or not aligned to its type.");
+    }
     for (size_t i = 0; i < bindings.size(); ++i)
         for (size_t j = 0; j < bindings.size(); ++j) {
             if (i == j || !(bindings[i].access & PC_ACCESS_WRITE) || !overlap(bindings[i].tensor, bindings[j].tensor)) continue;

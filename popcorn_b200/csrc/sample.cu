@@ -196,7 +196,7 @@ struct Weight {
         e = fma(e, x, 1.0830424696249145e-02);
         e = fma(e, x, 1.0);
         const double t = tab[(n & 63) * 16];
-        const double s = __hiloint2double(__double2hiint(t) + n * 16384, __double2loint(t));
+        const double s = __hiloint2double(__double2hiint(t) + int(unsigned(n) * 16384u), __double2loint(t));
         return fma(e, s, 4503599627370496.0) - 4503599627370496.0;
     }
     __device__ __forceinline__ u64 operator()(float l) const { return is_live(l) ? u64(of_live(l)) : 0; }

@@ -226,3 +226,23 @@ def test_lengths_that_overflow_are_refused():
     R = a["block_table"].shape[0]
     pc.Kernels.PagedAttention(**dict(a, block_table=fake([R, W], ptr=1 << 30)))
     refused(E.tensorShapeMismatch, pc.Kernels.PagedAttention, **dict(a, block_table=fake([R, W + 1], ptr=1 << 30)))
+
+
+@pytest.mark.parametrize("creator,args", [
+    (pc.Kernels.PagedBatchBuild, batch_args), (pc.Kernels.PagedQKVScatter, scatter_args),
+    (pc.Kernels.PagedAttention, attention_args), (pc.Kernels.Sample, sample_args)])
+def test_addresses_are_checked(creator, args):
+    """No memory, or an address that is no multiple of the type's size, is refused for every tensor."""
+    a = args()
+    creator(**a)
+    tensors = {n: t for n, t in a.items() if isinstance(t, pc.Tensor)}
+    assert len(tensors) >= 5
+    for name, t in tensors.items():
+        refused(E.tensorShapeMismatch, creator, **dict(a, **{name: fake(t.shape, t.dtype, 0)}))
+        refused(E.tensorShapeMismatch, creator, **dict(a, **{name: fake(t.shape, t.dtype, 0x7E0000000001)}))
+
+
+@pytest.mark.parametrize("shape", [(1 << 40, 1 << 40), (1 << 62, 4)])
+def test_sizes_that_overflow_are_refused(shape):
+    refused(E.tensorShapeMismatch, pc.Kernels.Sample, **sample_args(logits=fake(shape, D.bf16, 1 << 40)))
+    refused(E.tensorShapeMismatch, pc.Kernels.PagedBatchBuild, **batch_args(block_table=fake(shape, D.i32, 1 << 40)))
