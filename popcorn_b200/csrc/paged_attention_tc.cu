@@ -25,11 +25,12 @@
 // product reads it as its A operand, so it never passes through shared
 // memory; one group's loads and waits pass under the other's exponentials. A
 // ring slot holds 8-key groups of [Hd/64][8 keys][128 B], so any page size
-// that is a multiple of 8 gives one layout (group stride Hd/64 KB) and the two
-// halves of a tile in neighbouring slots are one operand.
+// that is a multiple of 8 gives one layout (group stride Hd/64 KB). At Hd 256
+// a tile takes two slots: K by columns, V by rows, the summed axis of either
+// product, so neither minds where in the ring its halves lie.
 //
 // What bounds it. Decoding: HBM; 32 requests of up to 8192 keys, 8 KV heads
-// of 256: 216 us in a row (5.3 TB/s), 250 with cold lengths and tables; a
+// of 256: 212 us in a row (5.4 TB/s), 250 with cold lengths and tables; a
 // single request of 4096 keys is all latency (27 us; a CTA's first product
 // comes some 12 us after its start: plan 7, look-ups and loads 5). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
 // tile) nor the tensor cores (as many), but the chain product, look at a
@@ -37,8 +38,11 @@
 // flight: 2250 clocks a tile at Hd 128 (32 % of the tensor cores' time; a
 // window of 4096 and 4 sinks, 2000 tokens of 32 heads: 210 us, 623 TFLOP/s of
 // visible pairs' work). Tiles of 64 keys, twice as many in flight, cost the
-// loads' warp as much each as those of 128: 315 us. Holding a half of S in
-// registers over the wait for the max spills: 250 us.
+// loads' warp as much each as those of 128: 315 us. Both groups on the halves
+// of one tile, which shortens the chain: 235 us, and no less at Hd 256, where
+// shared memory's bandwidth (operands and copies: 320 KB a tile, 2500 clocks)
+// is near. Holding a half of S in registers over the wait for the max spills:
+// 250 us.
 //
 // The running max is kept until it grows by more than 2^8 (P <= 256 then; O
 // and l use the same max, so O / l is exact for any); it goes from group to
@@ -86,7 +90,9 @@ struct Shape {
     static constexpr int NS = HD == 256 ? 2 : 3;  // S accumulators: NS * 128 + HD <= 512 columns
     static constexpr int GROUP = ATOMS * 1024;    // bytes of 8 keys
     static constexpr int HALVES = HD == 256 ? 2 : 1;  // ring slots of a 128-key tile
-    static constexpr int KEYS = kN / HALVES;          // keys of a slot
+    static constexpr int KEYS = kN / HALVES;          // V rows of a slot: half of the tile's rows at Hd 256
+    static constexpr int K_ATOMS = ATOMS / HALVES;    // K: all rows, half of their columns, so that Q.K^T has N = 128
+    static constexpr int K_GROUP = K_ATOMS * 1024;
     static constexpr int SLOT = KEYS / 8 * GROUP;
     static constexpr int NSLOT = HD == 256 ? 5 : (HD == 128 ? 6 : 10);
     // Warp 0's notes on items and units, a ring. It writes note j with K(j - 1)
@@ -341,11 +347,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 }
 
 // One ring slot: `n` boxes of `step` bytes.
-__device__ __noinline__ void load_boxes(uint32_t dst, uint32_t bar, uint32_t bytes, const CUtensorMap* map, const int* group,
-                                        int n, uint32_t step) {
+__device__ __noinline__ void load_boxes(uint32_t dst, uint32_t bar, uint32_t bytes, const CUtensorMap* map, int atom,
+                                        const int* group, int n, uint32_t step) {
     mbar_expect_tx(bar, bytes);
 #pragma unroll 1
-    for (int b = 0; b < n; ++b) tma_load_4d(dst + b * step, map, 0, 0, 0, group[b], bar);
+    for (int b = 0; b < n; ++b) tma_load_4d(dst + b * step, map, 0, 0, atom, group[b], bar);
 }
 
 // A from tensor memory (16-bit pairs, a row a lane), B from shared memory.
@@ -786,12 +792,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     };
     const int boxes = kN / 8 / a.box_groups;  // TMA boxes of a tile
     // One slot's boxes, issued one by one by lane 0: `to` gets the bytes.
-    auto put = [&](const int* group, int q, uint64_t* to, const CUtensorMap* map) {
+    auto put = [&](const int* group, int n, uint32_t step, int atom, int q, uint64_t* to, const CUtensorMap* map) {
         const int slot = q % NSLOT;
         if (!wait_bar(empty[slot], (uint32_t(q / NSLOT) & 1u) ^ 1u, s_abort)) return false;
         if (lane == 0)
-            load_boxes(smem_u32(ring) + slot * S::SLOT, smem_u32(to ? to : &full[slot]), S::SLOT, map, group, boxes / H,
-                       a.box_groups * S::GROUP);
+            load_boxes(smem_u32(ring) + slot * S::SLOT, smem_u32(to ? to : &full[slot]), S::SLOT, map, atom, group, n, step);
         __syncwarp();
         return true;
     };
@@ -887,7 +892,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     ++items;
                 }
 #pragma unroll 1
-                for (int h = 0; h < H && ok; ++h) ok = put(note.group + h * (boxes / H), k_pos(j) + h, nullptr, &map_k);
+                for (int h = 0; h < H && ok; ++h)
+                    ok = put(note.group, boxes, a.box_groups * S::K_GROUP, h * S::K_ATOMS, k_pos(j) + h, nullptr, &map_k);
             }
         }
         if (ok) ok = wait_bar(unit_free[j % kNotes], (uint32_t(j / kNotes) & 1u) ^ 1u, s_abort);
@@ -906,14 +912,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (!ok || (note.flags & kStop)) break;
 #pragma unroll 1
             for (int h = 0; h < H && ok; ++h)
-                ok = put(note.group + h * (boxes / H), v_pos(j) + h,
+                ok = put(note.group + h * (boxes / H), boxes / H, a.box_groups * S::GROUP, 0, v_pos(j) + h,
                          note.flags & (kLook << h) ? &look[looks++ % kNotes] : nullptr, &map_v);
         }
         if (!ok) s_abort = 1;
     } else if (warp == 1) {
         // ---- S = Q.K^T ----
         if (lane == 0) {
-            constexpr uint32_t idesc_s = make_idesc(BF, kM, kN, false), idesc_h = make_idesc(BF, kM, kN / 2, false);
+            constexpr uint32_t idesc_s = make_idesc(BF, kM, kN, false);
             const uint32_t q_base = smem_u32(sq), ring_a = smem_u32(ring);
             bool ok = true;
             for (int j = 0, k = 0; ok; ++j) {
@@ -929,18 +935,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 if (ok && H > 1) ok = wait_one(full[s1], uint32_t(q1 / NSLOT) & 1u, s_abort);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t k0 = ring_a + s0 * S::SLOT, k1 = ring_a + s1 * S::SLOT;
                 const uint32_t d = tmem + uint32_t(buf * kN);
-                // one N = 128 product, or two of 64 where the tile wraps round the ring
-                const bool one = H == 1 || s1 == s0 + 1;
+                uint64_t da = smem_desc_sw128(q_base);
 #pragma unroll 1
-                for (int h = 0; h < (one ? 1 : 2); ++h) {
-                    uint64_t da = smem_desc_sw128(q_base), db = desc_k(h ? k1 : k0, S::GROUP);
-                    const uint32_t to = d + uint32_t(h * (kN / 2)), idesc = one ? idesc_s : idesc_h;
+                for (int h = 0; h < H; ++h) {
+                    uint64_t db = desc_k(ring_a + (h ? s1 : s0) * S::SLOT, S::K_GROUP);
 #pragma unroll 1
-                    for (int at = 0; at < ATOMS; ++at) {
+                    for (int at = 0; at < S::K_ATOMS; ++at) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) tc_mma(to, da + 2 * kk, db + 2 * kk, idesc, (at | kk) ? 1u : 0u);
+                        for (int kk = 0; kk < 4; ++kk) tc_mma(d, da + 2 * kk, db + 2 * kk, idesc_s, (h | at | kk) ? 1u : 0u);
                         da += S::Q_BLOCK >> 4;
                         db += 1024 >> 4;
                     }
@@ -1053,8 +1056,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int quarter = warp & 3;  // TMEM lanes this warp may access
         const int row = quarter * 32 + lane;
         const uint32_t lane_off = uint32_t(quarter * 32) << 16;
-        const int ti = row / a.group, gi = row % a.group;
-        Item it;
         int row_lo = 0, row_hi = 0, row_sink = 0;  // keys that the row sees: [0, sink), [lo, hi)
         bool ok = true, valid = false, live = false;
         int k = -1;
@@ -1077,9 +1078,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 flags = (next & kNextFirst ? kFirst : 0) | (next & kNextLast ? kLast : 0);
             }
             if (flags & kFirst) {
+                Item it;
                 ok = item(++k, it);
                 if (!ok) break;
-                const int rows = it.ntok * a.group;
+                const int ti = row / a.group, rows = it.ntok * a.group;
                 valid = row < rows;
                 live = quarter * 32 < rows;  // some row of the warp is there
                 const Keys v = keys_of(p, it.len, it.pos0 + ti);
@@ -1173,6 +1175,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (ok && (j & 1) != w) ok = wait_bar(m_ready[w ^ 1][quarter], uint32_t(j >> 1) & 1u, s_abort);
             if (!ok) break;
             tc_fence_after();
+            const Item it = s_item[k % kNotes];  // (kept until the next item's products have passed this point)
+            const int ti = row / a.group, gi = row % a.group;
             const float last_m = s_m[row];
             if (m != last_m && m != -INFINITY) l *= ex2(m - last_m);
             // the group without the last tile gives its share, the other one the sum of both
@@ -1316,9 +1320,10 @@ cudaError_t run_tc(const PagedAttention& p, const PagedScratch& sc, cudaStream_t
     {
         const cuuint64_t dims[4] = {64, 8, HD / 64, cuuint64_t(a.groups)};
         const cuuint64_t strides[3] = {HD * 2, 128, 8 * HD * 2};
-        const cuuint32_t box[4] = {64, 8, HD / 64, cuuint32_t(a.box_groups)};
-        if (!encode_map(&mk, p.k_pages, p.dtype, dims, strides, box) ||
-            !encode_map(&mv, p.v_pages, p.dtype, dims, strides, box))
+        const cuuint32_t k_box[4] = {64, 8, Shape<HD>::K_ATOMS, cuuint32_t(a.box_groups)};
+        const cuuint32_t v_box[4] = {64, 8, HD / 64, cuuint32_t(a.box_groups)};
+        if (!encode_map(&mk, p.k_pages, p.dtype, dims, strides, k_box) ||
+            !encode_map(&mv, p.v_pages, p.dtype, dims, strides, v_box))
             return cudaErrorInvalidValue;
     }
     static DeviceOnce once;
