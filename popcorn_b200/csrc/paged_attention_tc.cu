@@ -30,7 +30,7 @@
 // product, so neither minds where in the ring its halves lie.
 //
 // What bounds it. Decoding: HBM; 32 requests of up to 8192 keys, 8 KV heads
-// of 256: 212 us in a row (5.4 TB/s), 250 with cold lengths and tables; a
+// of 256: 212 us in a row (5.4 TB/s), 237 alone, its prologue in sight; a
 // single request of 4096 keys is all latency (27 us; a CTA's first product
 // comes some 12 us after its start: plan 7, look-ups and loads 5). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
 // tile) nor the tensor cores (as many), but the chain product, look at a
