@@ -7,7 +7,7 @@
 // 128-key tiles that some row of it sees: those of the sink tokens, then
 // those from the first row's window start to the last row's position.
 // Every CTA of one wave takes an equal run of consecutive units (an item also
-// counts for one, its epilogue's share), cutting an item where its run ends
+// counts for four, its ends' share), cutting an item where its run ends
 // unless the item's own end is near: ragged lengths, long contexts with one
 // token and long chunks all fill the GPU. The pieces' (m, l, O) go to scratch
 // and a second kernel joins them in order (the cuts depend on the lengths
@@ -30,7 +30,7 @@
 // product, so neither minds where in the ring its halves lie.
 //
 // What bounds it. Decoding: HBM; 32 requests of up to 8192 keys, 8 KV heads
-// of 256: 212 us in a row (5.4 TB/s), 237 alone, its prologue in sight; a
+// of 256: 207 us in a row (5.6 TB/s), 226 alone, its prologue in sight; a
 // single request of 4096 keys is all latency (27 us; a CTA's first product
 // comes some 12 us after its start: plan 7, look-ups and loads 5). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
 // tile) nor the tensor cores (as many), but the chain product, look at a
@@ -497,12 +497,14 @@ __device__ __noinline__ void make_plan(const TcArgs& a, long long* cum, long lon
             }
             units += scan[x];
         }
-        // With runs long enough, an item counts for its epilogue too, and cuts keep clear of its ends.
-        const int extra = units >= 16ll * gridDim.x ? 1 : 0;
+        // With runs long enough, an item counts for its epilogue and its masked tiles too, as four units, and cuts keep
+        // clear of its ends. (1, 2, 3, 4, 6: a mixed step of 13 requests 115, 110, 104, 102, 100 us, 32 decoding ones 213,
+        // 209, 206, 207, 209, prompts alone 128, 133, 130, 134, 135.)
+        const int extra = units >= 16ll * gridDim.x ? 4 : 0;
         run += extra * run_items;
 #pragma unroll 1
         for (int r = r0; r < r1; ++r) {
-            run += cum[r + 1] + (extra ? (long long)tiles_of(a, req(p, r)) * p.Nkv : 0);
+            run += cum[r + 1] + extra * ((long long)tiles_of(a, req(p, r)) * p.Nkv);
             cum[r + 1] = run;
         }
         if (tid == 0) {

@@ -264,6 +264,23 @@ def test_attention_long_contexts(pc, enc, dt, hd, page):
         check_attention(pc, enc, case, keys, dt, pc.AttentionMask.causal_sliding_window(1000), WINDOW, 1000, 64)
 
 
+@pytest.mark.parametrize("dt,hd,page", [("bf16", 256, 64), ("f16", 128, 16), ("bf16", 64, 8)])
+@pytest.mark.parametrize("new,keys", [
+    ([700, 1, 1, 130, 0, 1, 1], [6000, 9000, 12000, 3001, 77, 500, 1]),  # chunks and single tokens
+    ([1] * 40, [1900 + 13 * i for i in range(40)]),                      # single tokens alone
+    ([257] * 23, [257 + 40 * i for i in range(23)]),                     # many short items
+])
+def test_attention_long_runs(pc, enc, dt, hd, page, new, keys):
+    """Steps with more than 16 tiles of 128 keys for each SM: items then count for more than their tiles."""
+    nq, nkv = 8, 4
+    tokens = 128 // (nq // nkv)  # of an item
+    tiles = sum(nkv * -(-(k - n + min(t + tokens, n)) // 128) for n, k in zip(new, keys) for t in range(0, n, tokens))
+    assert tiles > 16 * torch.cuda.get_device_properties(0).multi_processor_count
+    case = attention_case(hd + len(new), new, keys, nq, nkv, hd, page, dt)
+    check_attention(pc, enc, case, keys, dt, pc.AttentionMask.causal, CAUSAL, 0, 0)
+    check_attention(pc, enc, case, keys, dt, pc.AttentionMask.causal_sliding_window(3000), WINDOW, 3000, 10)
+
+
 @pytest.mark.parametrize("dt,hd,page", [("bf16", 256, 16), ("f16", 128, 64), ("bf16", 64, 32), ("f32", 64, 16)])
 def test_attention_masked_poison(pc, enc, dt, hd, page):
     """NaN and infinities in keys and values reach the rows that see them, and no other."""
