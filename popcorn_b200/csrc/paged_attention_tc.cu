@@ -82,6 +82,7 @@ constexpr int kPtThreads = 416;  // warps: 0 Q and K loads, 1 Q.K^T, 2 V loads, 
 constexpr int kSoftWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 of the growth of a row's max that is let pass
+constexpr float kFar = 4194304.f;  // 2^22: maxima below it are within 1/4 of their unrounded product
 constexpr uint32_t kTmem = 512;
 
 template <int HD>
@@ -645,6 +646,30 @@ __device__ __noinline__ void hide_scores(uint32_t at, int key0, int lo, int hi, 
     tmem_wait_st();
 }
 
+// A tile's weights 2^(c s - m) over its scores, their sum added to l, with the product rounded as the row's maximum was: so
+// far from zero (kFar) one that is not rounded lies whole powers of two above or below it.
+template <class T>
+__device__ __noinline__ float weigh_far(uint32_t at, float c, float m, float l) {
+#pragma unroll 1
+    for (int h = 0; h < kN; h += 64) {
+        float pk[32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float s[32];
+            tmem_ld32(at + h + 32 * i, s);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                const float x = ex2(__fsub_rn(__fmul_rn(s[e], c), m)), y = ex2(__fsub_rn(__fmul_rn(s[e + 1], c), m));
+                l += x + y;
+                pk[16 * i + e / 2] = __uint_as_float(cvt_pair<T>(x, y));
+            }
+        }
+        tmem_st32(at + h, pk);
+    }
+    tmem_wait_st();
+    return l;
+}
+
 __device__ __noinline__ void scale_columns(uint32_t at, int columns, float f) {
 #pragma unroll 1
     for (int c = 0; c < columns; c += 32) {
@@ -1126,7 +1151,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 const bool first = flags & kFirst;
                 const float before = first ? -INFINITY : s_m[row];
                 float now = before;
-                if (valid && mx > before + kGrow) now = mx;
+                if (valid && mx > __fadd_rd(before, kGrow)) now = mx;
                 s_m[row] = now;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&m_ready[w][quarter]));
@@ -1134,7 +1159,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     if (m != -INFINITY) l *= ex2(m - now);
                     m = now;
                 }
-                if (live) {
+                if (live && __any_sync(0xffffffffu, fabsf(m) >= kFar && m != -INFINITY)) {
+                    l = weigh_far<T>(at_s, a.c, m == -INFINITY ? 0.f : m, l);
+                } else if (live) {
                     const float mu = m == -INFINITY ? 0.f : m;
                     const float2 c2 = make_float2(a.c, a.c), m2 = make_float2(-mu, -mu);
                     float2 sum0 = make_float2(l, 0.f), sum1 = make_float2(0.f, 0.f);
