@@ -44,11 +44,13 @@
 // is near. Holding a half of S in registers over the wait for the max spills:
 // 250 us.
 //
-// The running max is kept until it grows by more than 2^8 (P <= 256 then; O
-// and l use the same max, so O / l is exact for any); it goes from group to
-// group with the tiles, warp to warp. P is rounded to
-// the type once: as far from the exact weights as the output's own rounding
-// is from the exact output (half a step each); sums, m, l and O are fp32.
+// The running max is kept until P would pass 2^8 (2^15 in f16; O and l use
+// the same max, so O / l is exact for any); it goes from group to group with
+// the tiles, warp to warp. P is rounded to the type once, as the second
+// product's operand: half a step of each weight that is a normal number there
+// (all of bf16's; in f16 those above 2^-25 of the row's largest, see Weights),
+// so that it moves a row by half a step of sum p |v| / l at most. l adds the
+// weights as they were before it; m, l and O are fp32.
 //
 // Keys that no row of the item sees are never loaded (zero-filled boxes, so
 // freed pages may hold anything). In tiles that cross a mask edge V rows that
@@ -81,9 +83,18 @@ constexpr int kN = 128;          // keys of a unit
 constexpr int kPtThreads = 416;  // warps: 0 Q and K loads, 1 Q.K^T, 2 V loads, 3 masked V, 4-11 softmax, 12 P.V
 constexpr int kSoftWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kGrow = 8.0f;  // log2 of the growth of a row's max that is let pass
 constexpr float kFar = 4194304.f;  // 2^22: maxima below it are within 1/4 of their unrounded product
 constexpr uint32_t kTmem = 512;
+
+// The weights P = 2^(c S - m) that the type holds. m is set to a row's max less START (the largest weight is then
+// 2^START) and kept until a weight would pass 2^TOP. bf16 has the exponents of fp32: any START does. f16 is subnormal below
+// 2^-14 and ends at 2^16: START = 11 keeps weights down to 2^-25 of the largest to half a step (2^-11) of their own size,
+// and smaller ones to 2^-36 of the largest. (START = 0 and TOP = 8 lost 40000 keys of 2^-25 each, 1.1e-3 of a row.)
+template <class T>
+struct Weights {
+    static constexpr float START = T::code == TBF16::code ? 0.f : 11.f;
+    static constexpr float TOP = T::code == TBF16::code ? 8.f : 15.f;
+};
 
 template <int HD>
 struct Shape {
@@ -1151,7 +1162,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 const bool first = flags & kFirst;
                 const float before = first ? -INFINITY : s_m[row];
                 float now = before;
-                if (valid && mx > __fadd_rd(before, kGrow)) now = mx;
+                if (valid && mx > __fadd_rd(before, Weights<T>::TOP)) now = __fsub_ru(mx, Weights<T>::START);
                 s_m[row] = now;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&m_ready[w][quarter]));
