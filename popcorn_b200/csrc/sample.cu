@@ -65,6 +65,7 @@ constexpr int kListK = 512;
 // 14.2 us against 15.2, 18.9 and 16.9; k = 200: 18.3, 20.3 and 18.9 against 17.5, 20.3 and 18.7).
 constexpr int kFew = 192;
 constexpr int kOneBits = 42;
+constexpr int64_t kMostTokens = (1 << 21) - 32768;  // of a CTA: sums of a thread's weights are exact in a double (see of_live)
 constexpr double kOne = 4398046511104.0;  // 2^42
 
 struct Pick {
@@ -185,7 +186,8 @@ struct Weight {
     // 2^42 exp((l - l_max) / T) of a live token, to the nearest whole number. With k = 64 log2 of the exponential and n the
     // integer next to it: 2^(n / 64), from a table and an exponent, times 2^((k - n) / 64), |k - n| <= 1/2, by its series
     // to the fourth power (the fifth is below 2^-44). Adding 1.5 2^52 or 2^52 rounds a double to a whole number. (A
-    // thread's share of a row, up to 2^11 of them, still sums exactly in a double.)
+    // thread's share of a row, up to 2^11 of them, still sums exactly in a double: of kMostTokens, at whatever alignment, a
+    // warp has 64512 and a lane at most 2018.)
     __device__ __forceinline__ double of_live(float l) const {
         const double d = double(l) - top;
         const double r = fma(d, c64, 6755399441055744.0);
@@ -1197,6 +1199,8 @@ cudaError_t run_sample(const Sample& p, cudaStream_t s) {
     auto chunk_of = [&](int c) { return ((p.V + c - 1) / c + 7) / 8 * 8; };
     int C = 1;
     while (C < 8 && p.rows * (C + 1) <= sms && chunk_of(C) > 4096) ++C;
+    // (more only for rows near 2^21; a cluster of two takes twice as many CTAs for half of the time each)
+    while (chunk_of(C) > kMostTokens) ++C;
     const int64_t chunk = chunk_of(C);
     const bool resident = size_t(chunk) * Elem<T>::bytes <= room;
     const size_t smem = sizeof(Shared) + (resident ? size_t(chunk) * Elem<T>::bytes + 16 : 0);
