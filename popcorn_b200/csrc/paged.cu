@@ -25,10 +25,13 @@ namespace {
 // most kMaxRequests) and keeps N, P and c in shared memory; after a cluster
 // barrier — the outputs may be the inputs — the cluster's threads write the
 // requests' rows, the new table entries and the tokens, each finding its
-// request by binary search, four neighbouring tokens a thread. Latency-bound:
-// 5.6 us for 32 decoding requests, 12 us for 509 prompts of 178000 tokens
-// (15 us with a search a token). One CTA up to kOneCtaTokens tokens, eight for
-// more (4096 tokens: 4.7 and 5.2 us, 6144: 5.7 and 5.3, 16384: 9.6 and 5.5).
+// request by binary search: a token a thread where there are threads enough,
+// else four neighbouring ones. Latency-bound: 3.9 us for 32 decoding requests
+// (5.6 with four tokens a thread, whose look-ups follow one another), 12 us
+// for 509 prompts of 178000 tokens (15 with a search a token). One CTA up to
+// kOneCtaTokens tokens, eight for more (2048 tokens of a prompt: 4.0 with one
+// and 4.1 with eight, 4096 of eight prompts: 4.6 and 4.4, 6695 of thirteen:
+// 6.0 and 4.4).
 constexpr int kBuildThreads = 1024;
 constexpr int64_t kOneCtaTokens = 4096;
 constexpr int kBuildCluster = 8;
@@ -46,6 +49,60 @@ __device__ __forceinline__ int find_owner(const int32_t* a, int n, int32_t x) {
         else hi = mid;
     }
     return lo;
+}
+
+// Positions and slots of the step's token rows, N neighbouring ones a thread: one search for them, and one page look-up unless
+// a page or a request ends among them.
+template <int N>
+__device__ __forceinline__ void write_tokens(const PagedBatch& p, const int32_t* start, const int32_t* pstart,
+                                             const int32_t* cached, int fail, int32_t total, int64_t head, int gt, int gn) {
+    const uint32_t ps = uint32_t(p.ps);
+    const bool wide = N == 4 && ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.slots)) & 15u) == 0;
+    for (int64_t t0 = N * int64_t(gt); t0 < p.T; t0 += N * int64_t(gn)) {
+        int32_t position[N], slot[N];
+        int r = t0 < total ? find_owner(start, fail, int32_t(t0)) : 0;
+        uint32_t pos = 0, pg = 0, off = 0;
+        int64_t page = -1;
+        bool look = true;  // (pos, pg and off are new)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            position[j] = 0;
+            slot[j] = -1;
+            const int64_t t = t0 + j;
+            if (t >= total) continue;
+            if (j == 0 || t >= start[r + 1]) {
+                while (j > 0 && t >= start[r + 1]) ++r;
+                pos = uint32_t(cached[r]) + uint32_t(int32_t(t) - start[r]);
+                pg = pos / ps;
+                off = pos - pg * ps;
+                look = true;
+            }
+            if (look) {
+                const uint32_t before = (uint32_t(cached[r]) + (ps - 1)) / ps;
+                page = pg < before ? p.table[int64_t(r) * p.W + pg] : p.free_pages[head + pstart[r] + (pg - before)];
+            }
+            const int64_t sl = page * ps + off;
+            position[j] = int32_t(pos);
+            slot[j] = page >= 0 && sl <= 0x7fffffffll ? int32_t(sl) : -1;
+            ++pos;
+            look = ++off == ps;
+            if (look) {
+                off = 0;
+                ++pg;
+            }
+        }
+        if constexpr (N == 4) {
+            if (wide && t0 + 4 <= p.T) {
+                *reinterpret_cast<int4*>(p.positions + t0) = make_int4(position[0], position[1], position[2], position[3]);
+                *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+                continue;
+            }
+        }
+        for (int j = 0; j < N && t0 + j < p.T; ++j) {
+            p.positions[t0 + j] = position[j];
+            p.slots[t0 + j] = slot[j];
+        }
+    }
 }
 
 __global__ void __launch_bounds__(kBuildThreads) paged_batch_build_kernel(const PagedBatch p) {
@@ -152,52 +209,8 @@ __global__ void __launch_bounds__(kBuildThreads) paged_batch_build_kernel(const 
         const long long before = (static_cast<long long>(cached[r]) + p.ps - 1) / p.ps;
         p.table[int64_t(r) * p.W + before + (i - pstart[r])] = p.free_pages[head + i];
     }
-    // Four neighbouring tokens a thread: one search, and one page look-up unless a page or a request ends among them.
-    const uint32_t ps = uint32_t(p.ps);
-    const bool wide = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.slots)) & 15u) == 0;
-    for (int64_t t0 = 4 * int64_t(gt); t0 < p.T; t0 += 4 * int64_t(gn)) {
-        int32_t position[4], slot[4];
-        int r = t0 < total ? find_owner(start, fail, int32_t(t0)) : 0;
-        uint32_t pos = 0, pg = 0, off = 0;
-        int64_t page = -1;
-        bool look = true;  // (pos, pg and off are new)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            position[j] = 0;
-            slot[j] = -1;
-            const int64_t t = t0 + j;
-            if (t >= total) continue;
-            if (j == 0 || t >= start[r + 1]) {
-                while (t >= start[r + 1]) ++r;
-                pos = uint32_t(cached[r]) + uint32_t(int32_t(t) - start[r]);
-                pg = pos / ps;
-                off = pos - pg * ps;
-                look = true;
-            }
-            if (look) {
-                const uint32_t before = (uint32_t(cached[r]) + (ps - 1)) / ps;
-                page = pg < before ? p.table[int64_t(r) * p.W + pg] : p.free_pages[head + pstart[r] + (pg - before)];
-            }
-            const int64_t sl = page * ps + off;
-            position[j] = int32_t(pos);
-            slot[j] = page >= 0 && sl <= 0x7fffffffll ? int32_t(sl) : -1;
-            ++pos;
-            look = ++off == ps;
-            if (look) {
-                off = 0;
-                ++pg;
-            }
-        }
-        if (wide && t0 + 4 <= p.T) {
-            *reinterpret_cast<int4*>(p.positions + t0) = make_int4(position[0], position[1], position[2], position[3]);
-            *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-        } else {
-            for (int j = 0; j < 4 && t0 + j < p.T; ++j) {
-                p.positions[t0 + j] = position[j];
-                p.slots[t0 + j] = slot[j];
-            }
-        }
-    }
+    if (p.T <= gn) write_tokens<1>(p, start, pstart, cached, fail, total, head, gt, gn);
+    else write_tokens<4>(p, start, pstart, cached, fail, total, head, gt, gn);
 }
 
 // ---- PagedQKVScatter -------------------------------------------------------
