@@ -128,7 +128,8 @@ PC_API const char* pc_library_function_name(const pc_library* library, int index
 /* ---- scratch protocol (Sources/Popcorn/KernelResources.swift:5-36) ------ */
 
 /* KernelScratchAllocator.borrowTemporaryBuffer(length:) / release. borrow
- * returns 0 and a device pointer of at least `length` bytes, and sets
+ * returns 0 and a device pointer of at least `length` bytes, aligned to 16
+ * bytes (as an allocation's start is), and sets
  * *was_reused when the buffer may hold earlier writes in the same encoder
  * (KernelTemporaryBuffer.wasReused, KernelResources.swift:14-20). A
  * non-zero return aborts the encode with that status. release may be NULL;

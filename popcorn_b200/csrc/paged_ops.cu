@@ -3,6 +3,7 @@
 // in paged.cu, paged_attention*.cu and sample.cu.
 #include <memory>
 
+#include "common.cuh"
 #include "launch.hpp"
 #include "popcorn.hpp"
 
@@ -233,6 +234,8 @@ public:
         const int ctas = enc.sm_count();
         const int64_t words = int64_t((launch::paged_attention_scratch_bytes(p, ctas) + 3) / 4);
         enc.with_temporaries({{{words}, PC_F32}}, [&](const std::vector<Tensor>& t) {
+            want(launch::aligned16(t[0].data()), PC_ERR_TENSOR_ALLOCATION_FAILED,
+                 "PagedAttention needs scratch memory that is aligned to 16 bytes.");
             const launch::PagedScratch sc{t[0].data(), ctas};
             std::vector<Binding> first = b_;
             first.push_back({t[0], PC_ACCESS_WRITE});
