@@ -484,8 +484,15 @@ PC_API int pc_kernel_paged_qkv_scatter(const pc_tensor* qkv, const pc_tensor* sl
  * keys: causal j <= position; sliding window also position - j < window, or
  * j < sinks (the first `sinks` tokens stay visible; sinks > 0 only with that
  * mask); bidirectional all. KV head hq * Nkv / Nq, Hd <= 512, at most 2^30
- * keys a request, one float dtype. fp32 softmax and accumulation; a row
- * without a visible key is zero; rows of no request are left as they are.
+ * keys a request, one float dtype. Scores, softmax statistics and sums are
+ * fp32. At 16 bits, Hd 64, 128 or 256 and pages of a multiple of 8 rows the
+ * products run on the tensor cores, and each weight is rounded once to the
+ * dtype before it meets its value: an output is off by at most half a step of
+ * sum p |v| more than by its own rounding (f16: weights below 2^-25 of the
+ * row's largest by up to 2^-36 of it each). Every other case holds the weights
+ * in fp32. (pc_kernel_flash_attention keeps twice as many bits of its bf16
+ * weights.) A row without a visible key is zero; rows of no request are left
+ * as they are.
  * Values in keys that a row does not see never reach it, whatever they are.
  * Lengths are clamped to the tensors on the device; a page id outside the
  * pages is never read: it sets bit 5 of the device error word and its

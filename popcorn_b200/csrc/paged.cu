@@ -30,8 +30,7 @@ namespace {
 // (5.6 with four tokens a thread, whose look-ups follow one another), 12 us
 // for 509 prompts of 178000 tokens (15 with a search a token). One CTA up to
 // kOneCtaTokens tokens, eight for more (2048 tokens of a prompt: 4.0 with one
-// and 4.1 with eight, 4096 of eight prompts: 4.6 and 4.4, 6695 of thirteen:
-// 6.0 and 4.4).
+// and 4.1 with eight, 4096 of eight prompts: 4.6 and 4.4).
 constexpr int kBuildThreads = 1024;
 constexpr int64_t kOneCtaTokens = 4096;
 constexpr int kBuildCluster = 8;

@@ -1,6 +1,7 @@
 // paged_attention.cu — attention of the step's new tokens over a paged KV
-// cache: the form for every type, head dim, page size and alignment, and the
-// routing to the tensor-core kernel (paged_attention_tc.cu).
+// cache: the form for every type, head dim, page size and alignment. (16-bit
+// types at head dims 64, 128 and 256 over pages of a multiple of 8 rows have
+// the tensor-core kernel, paged_attention_tc.cu.)
 //
 // Token i of request r (n_r new tokens, s_r keys with them) sits at position
 // p = s_r - n_r + i and attends to the keys j of its request that its mask
@@ -8,8 +9,9 @@
 // (the first tokens stay visible); bidirectional j < s_r. Key j is row
 // j % ps of page block_table[r, j / ps]. Online softmax in fp32, one rounding
 // of O / l. A row without a visible key is zero. Tokens of no request keep
-// their rows. A page id outside the pages sets bit 5 of the device error
-// word and its keys are skipped.
+// their rows. A page id outside the pages is not read and sets bit 5 of the
+// device error word; its request's rows then mean nothing (here its keys are
+// skipped, the tensor-core kernel takes them as zeros).
 #include "async.cuh"
 #include "common.cuh"
 #include "dtype.cuh"
@@ -31,6 +33,12 @@ constexpr int kPaWarps = 4;
 // One CTA per (token, query head): four warps take the visible keys in turn,
 // a lane every 32nd element of the row; their states merge at the end. Only
 // visible rows are read, so nothing in a masked row can reach the output.
+// Simple, and far from its floor: every (token, head) reads its whole context,
+// a row at a time, with no reuse over a chunk's tokens or a group's heads. f32,
+// 8 / 4 heads of 256: one request of 4096 keys 2.2 to 4.3 ms, 4 prompts of 2048
+// 41 ms; 32 decoding at up to 8192 keys, 16 / 8 heads: 10 ms. 16-bit: 32
+// decoding, heads of 96, 3.7 ms; a windowed chunk of 2000 over pages of 100
+// rows 110 ms.
 template <class T>
 __global__ void __launch_bounds__(kPaThreads) paged_attention_any_kernel(const PagedAttention p) {
     constexpr int MAXE = 16;

@@ -30,13 +30,18 @@
 // product, so neither minds where in the ring its halves lie.
 //
 // What bounds it. Decoding: HBM; 32 requests of up to 8192 keys, 8 KV heads
-// of 256: 207 us in a row (5.6 TB/s), 226 alone, its prologue in sight; a
+// of 256: 208 us a launch (5.55 TB/s) for the first 40 ms after a rest, at
+// full clocks; 231 to 238 (4.9 TB/s) after that, where the 1000 W limit takes
+// the SMs from 1965 to some 1560 MHz (a copy then goes from 6.53 to 6.3 TB/s);
+// whether the inputs are the last launch's or others makes no difference. A
 // single request of 4096 keys is all latency (27 us; a CTA's first product
-// comes some 12 us after its start: plan 7, look-ups and loads 5). Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
+// comes some 12 us after its start: plan 7, look-ups and loads 5; only the
+// barriers' and tensor memory's set-up, 1 us, passes under the launch before).
+// Chunks: neither the MUFU's 16 exponentials a clock (1024 clocks a
 // tile) nor the tensor cores (as many), but the chain product, look at a
 // barrier, softmax, product of a tile, some 6700 clocks, over the NS tiles in
 // flight: 2250 clocks a tile at Hd 128 (32 % of the tensor cores' time; a
-// window of 4096 and 4 sinks, 2000 tokens of 32 heads: 210 us, 623 TFLOP/s of
+// window of 4096 and 4 sinks, 2000 tokens of 32 heads: 209 us, 641 TFLOP/s of
 // visible pairs' work). Tiles of 64 keys, twice as many in flight, cost the
 // loads' warp as much each as those of 128: 315 us. Both groups on the halves
 // of one tile, which shortens the chain: 235 us, and no less at Hd 256, where

@@ -36,9 +36,9 @@
 // Bound by instructions and, with few rows, by the chain of cluster barriers
 // (some 0.6 us each) and cold code; the HBM floor is far. One row of 256000
 // bf16, top-k 64: 11 us (all sorting and histogramming in full: 58). 131 rows
-// of 50257 f16, top-k 200: 18 us. 48 rows of 256000 f32, top-p 0.9: 78 us, 95
+// of 50257 f16, top-k 200: 17 us. 48 rows of 256000 f32, top-p 0.9: 75 us, 94
 // when the 49 MB come from HBM (a pass of weights more: 120; weights by exp():
-// 250).
+// 250); without a filter 48 and 62 us, greedy 30 and 45.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -69,8 +69,7 @@ constexpr int64_t kMostTokens = (1 << 21) - 32768;  // of a CTA: sums of a threa
 constexpr double kOne = 4398046511104.0;  // 2^42
 
 struct Pick {
-    u64 before_cnt, before_mass;  // of the tokens above the picked bin
-    u64 total_cnt, total_mass;    // of everything the histogram saw
+    u64 before_cnt, before_mass;  // of the tokens above the picked bin (of everything the histogram saw, if none is)
     uint32_t n;                   // tokens in the bin
     int bin;                      // -1: the prefix takes everything
 };
@@ -446,13 +445,13 @@ __device__ Pick pick_bin(const Cluster& cl, bool by_mass, double goal, u64 befor
         const u64 tc = before_cnt + sh->wsum[31], tm = before_mass + sh->wsum2[31];
         c += before_cnt + (warp ? sh->wsum[warp - 1] : 0);   // inclusive of this thread's bins
         m += before_mass + (warp ? sh->wsum2[warp - 1] : 0);
-        if (tid == 0) sh->pick = Pick{tc, tm, tc, tm, 0, -1};
+        if (tid == 0) sh->pick = Pick{tc, tm, 0, -1};
         __syncthreads();
         const u64 ec = c - c0 - c1, em = m - m0 - m1;  // before the first bin
         const double p0 = by_mass ? double(em) : double(ec), p1 = by_mass ? double(em + m0) : double(ec + c0),
                      p2 = by_mass ? double(m) : double(c);
-        if (p0 < goal && goal <= p1) sh->pick = Pick{ec, em, tc, tm, uint32_t(c0), 2 * tid};
-        else if (p1 < goal && goal <= p2) sh->pick = Pick{ec + c0, em + m0, tc, tm, uint32_t(c1), 2 * tid + 1};
+        if (p0 < goal && goal <= p1) sh->pick = Pick{ec, em, uint32_t(c0), 2 * tid};
+        else if (p1 < goal && goal <= p2) sh->pick = Pick{ec + c0, em + m0, uint32_t(c1), 2 * tid + 1};
         __syncthreads();
         const Pick got = sh->pick;
         if (tid < cl.C && tid > 0) cl.of(tid)->pick = got;
@@ -1193,9 +1192,9 @@ template <class T>
 cudaError_t run_sample(const Sample& p, cudaStream_t s) {
     const int sms = current_sm_count();
     const size_t room = 227 * 1024 - sizeof(Shared) - 16;  // (16: the row's own distance from a 16-byte border)
-    // CTAs a row: all SMs once with few rows, at least 4096 tokens each. (48 rows of 256000 f32: 3 CTAs, which read the
-    // row from L2 again, 120 us; 8, which hold it but are 2.6 waves, 189; 131 rows of 50257 f16: 1 CTA 20 us, 2 41 us; one
-    // row of 256000 bf16: 8 CTAs 22 us, 4 24, 1 44.)
+    // CTAs a row: all SMs once with few rows, at least 4096 tokens each. (48 rows of 256000 f32, top-p: 3 CTAs, which read
+    // the row from L2 again, 94 us, 2 as much, 1 154; 8, which hold it but are 2.6 waves, 134; 131 rows of 50257 f16,
+    // top-k: 1 CTA 18 us, 2 39; one row of 256000 bf16, top-k: 8 CTAs 11 us, 4 15, 1 20.)
     auto chunk_of = [&](int c) { return ((p.V + c - 1) / c + 7) / 8 * 8; };
     int C = 1;
     while (C < 8 && p.rows * (C + 1) <= sms && chunk_of(C) > 4096) ++C;
