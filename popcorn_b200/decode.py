@@ -300,7 +300,8 @@ class PagedStack:
         the requests' last rows -> Matmul (LM head) -> Sample
 
     A step reads `added` [requests] (new tokens each), `ids` [tokens] (their
-    token ids, request after request), `uniform` [requests] (numbers in
+    token ids, request after request; the rows after them: any ids of the
+    vocabulary), `uniform` [requests] (numbers in
     [0, 1)) and the sampling parameters `temperature`, `top_k`, `top_p` and
     `min_p` [requests]; it keeps `seq_lens`, `block_table` and `free_head` on
     the device, and leaves `logits` [requests, vocab], `next` [requests] and
